@@ -80,12 +80,31 @@ _SIGNATURES = {
     "qb_linear_ce_grad": [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
     "qb_pack_segment_size": [],
     "qb_adapter_pack": [_p, _i32, _i64, _p],
+    "qb_token_logprobs": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p],
+    "qb_token_logprobs_bwd": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p,
+                              _p, _p],
+    "qb_preference_config_size": [],
+    "qb_preference_workspace": [_i64, _i64],
+    "qb_preference_fwd": [_p, _p, _i32, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p],
+    "qb_preference_bwd": [_p, _p, _p, _i64, _i64, _p, _i32, _p],
+    "qb_policy_config_size": [],
+    "qb_policy_workspace": [_i64, _i64],
+    "qb_policy_fwd": [_p, _p, _p, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p,
+                      _p, _p],
+    "qb_policy_bwd": [_p, _p, _i64, _p, _i64, _i64, _p, _i32, _p],
+    "qb_grad_norm_workspace": [_i64],
+    "qb_grad_norm": [_p, _p, _p, _i64, _i32, _p, _i64, _p, _p],
+    "qb_grad_clip": [_p, _p, _p, _i64, _i32, _p, _p, _i64, _p, _p],
 }
 _RESTYPE = {"qb_last_error": ctypes.c_char_p, "qb_nf4_double_quant_workspace": ctypes.c_int64,
             "qb_nf4_double_quant_noalloc_max_blocks": ctypes.c_int64,
             "qb_linear_ce_vocab_tiles": ctypes.c_int64,
             "qb_gemm_bf16_acc_f32_workspace": ctypes.c_int64,
-            "qb_pack_segment_size": ctypes.c_int64, "qb_mask_job_size": ctypes.c_int64}
+            "qb_pack_segment_size": ctypes.c_int64, "qb_mask_job_size": ctypes.c_int64,
+            "qb_preference_config_size": ctypes.c_int64,
+            "qb_preference_workspace": ctypes.c_int64,
+            "qb_policy_config_size": ctypes.c_int64, "qb_policy_workspace": ctypes.c_int64,
+            "qb_grad_norm_workspace": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -151,6 +170,11 @@ class KernelTimer:
 _timer = None
 
 
+def timing():
+    """True while a KernelTimer is active (a caller whose work figures cost time to add up asks)."""
+    return _timer is not None
+
+
 def call(name, *args, work=(0, 0), kernels=1):
     """Calls a C-ABI entry point; raises RuntimeError with the library's message on failure.
     `work` = (algorithmic bytes, flops) of the call and `kernels` the kernels it launches,
@@ -169,6 +193,18 @@ def call(name, *args, work=(0, 0), kernels=1):
     if status != 0:
         msg = lib.qb_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (status {status}): {msg}")
+
+
+def call_on(device, name, *args, work=(0, 0), kernels=1):
+    """call() with `device` as the current one and its current stream as the last argument: a
+    launch on a stream of another device than the current one is refused by the runtime."""
+    here = torch.cuda.current_device()
+    at = here if device.index is None else device.index
+    raw = torch._C._cuda_getCurrentRawStream(at)     # stream(device) without the Stream object
+    if at == here:
+        return call(name, *args, raw, work=work, kernels=kernels)
+    with torch.cuda.device(at):
+        return call(name, *args, raw, work=work, kernels=kernels)
 
 
 def tag(dtype):

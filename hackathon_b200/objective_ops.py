@@ -1,0 +1,364 @@
+"""The post-training ops as PyTorch operators (namespace `qlora_b200`, beside those of ops.py):
+
+    op                      computes                                          backward
+    token_logprobs          log-probability of each row's target token, the   token_logprobs_bwd
+                            row's entropy, (max, sum) of the row
+    token_logprobs_bwd      dlogits
+    preference              pairs' loss; rewards and each row's coefficient   preference_bwd
+    preference_bwd          dlogp = mask * coefficient * g
+    policy                  clipped policy loss + KL; its statistics, the     policy_bwd
+                            rows' weights, the unit gradient
+    policy_bwd              dlogp = unit gradient * row weight * g
+
+The functions users call (logprobs.py, preference.py, policy.py) check their arguments and bring
+them into the layouts these ops read. The kernels of an objective take a few microseconds at the
+sizes of a batch, so the host's part decides: the ops are registered with torch.library's
+define / impl and an autograd.Function of their own (a preference loss and its gradient took
+239 us of host time through torch.library.custom_op and its generated formula, against 70 us for
+an empty autograd.Function on the same machine), and small outputs share one allocation with the
+workspace.
+"""
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import NS
+
+F32 = torch.float32
+_library = torch.library.Library(NS, "FRAGMENT")
+_below_autograd = torch._C._AutoDispatchBelowAutograd
+
+
+def _register(schema, fake, function=None, grad_arg=0):
+    """Registers the decorated function as the CUDA kernel of the op `schema` declares, with its
+    fake implementation; `function`: the autograd.Function that calls it when the argument
+    numbered grad_arg asks for a gradient. Returns the op."""
+    name = schema[:schema.index("(")]
+
+    def register(kernel):
+        _library.define(schema)
+        _library.impl(name, kernel, "CUDA")
+        torch.library.register_fake(f"{NS}::{name}", fake, lib=_library)
+        op = getattr(getattr(torch.ops, NS), name).default
+        if function is not None:
+            def autograd(*args):
+                if torch.is_grad_enabled() and args[grad_arg].requires_grad:
+                    return function.apply(*args)
+                with _below_autograd():
+                    return op(*args)
+            _library.impl(name, autograd, "Autograd")
+        return op
+    return register
+
+
+class PreferenceConfig(ctypes.Structure):
+    _fields_ = [("beta", ctypes.c_double), ("label_smoothing", ctypes.c_double),
+                ("margin", ctypes.c_double), ("denominator", ctypes.c_double),
+                ("loss_type", ctypes.c_int32), ("length_normalized", ctypes.c_int32)]
+
+
+class PolicyConfig(ctypes.Structure):
+    _fields_ = [("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double),
+                ("delta", ctypes.c_double), ("kl_coef", ctypes.c_double),
+                ("denominator", ctypes.c_double), ("reduction", ctypes.c_int32),
+                ("pad", ctypes.c_int32)]
+
+
+# ------------------------------------------------------------------------------------------
+# log-probabilities of chosen tokens
+
+
+def row_layout(logits):
+    """(logits, rows, inner, outer stride, inner stride): row r of [..., V] logits starts at
+    (r // inner) * outer + (r % inner) * inner stride. Up to two leading dimensions of any
+    strides are read in place (a view that drops the last position, an expanded one); the rest
+    is copied first."""
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        logits = logits.contiguous()
+    if logits.dim() > 3 or logits.dim() == 1:
+        logits = logits.reshape(-1, logits.shape[-1])
+    if logits.dim() == 2:
+        return logits, logits.shape[0], 1, logits.stride(0), 0
+    b, s, _ = logits.shape
+    if b <= 1 or logits.stride(0) == s * logits.stride(1):
+        return logits, b * s, 1, logits.stride(1), 0
+    return logits, b * s, max(s, 1), logits.stride(0), logits.stride(1)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, temperature, with_entropy):
+        with _below_autograd():
+            logp, entropy, stats = token_logprobs(logits, target, temperature, with_entropy)
+        ctx.save_for_backward(logits, target, stats, entropy if with_entropy else None)
+        ctx.temperature, ctx.with_entropy = temperature, with_entropy
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*((stats,) if with_entropy else (entropy, stats)))
+        return logp, entropy, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, _g_stats):
+        logits, target, stats, entropy = ctx.saved_tensors
+        if not ctx.with_entropy:
+            g_entropy = None
+        if g_logp is None and g_entropy is None:
+            return None, None, None, None
+        return token_logprobs_bwd(logits, target, stats, entropy, g_logp, g_entropy,
+                                  ctx.temperature), None, None, None
+
+
+def _token_logprobs_fake(logits, target, temperature, with_entropy):
+    return (target.new_empty(target.shape, dtype=F32),
+            target.new_empty(target.shape if with_entropy else (0,), dtype=F32),
+            target.new_empty((target.numel(), 2), dtype=F32))
+
+
+@_register("token_logprobs(Tensor logits, Tensor target, float temperature, bool with_entropy) "
+           "-> (Tensor, Tensor, Tensor)", _token_logprobs_fake, _TokenLogprobs)
+def token_logprobs(logits, target, temperature, with_entropy):
+    z, rows, inner, so, si = row_layout(logits)
+    vocab, dev = logits.shape[-1], logits.device
+    logp = torch.empty(target.shape, dtype=F32, device=dev)
+    entropy = torch.empty(target.shape if with_entropy else (0,), dtype=F32, device=dev)
+    stats = torch.empty((rows, 2), dtype=F32, device=dev)
+    if rows:
+        tgt = target.contiguous()
+        _lib.call_on(dev, "qb_token_logprobs", z.data_ptr(), _lib.tag(z.dtype), rows, inner, so,
+                     si, vocab, tgt.data_ptr(), temperature, logp.data_ptr(),
+                     entropy.data_ptr() if with_entropy else None, stats.data_ptr(),
+                     work=(rows * (vocab * z.element_size() + 20), 0))
+    return logp, entropy, stats
+
+
+@_register("token_logprobs_bwd(Tensor logits, Tensor target, Tensor stats, Tensor? entropy, "
+           "Tensor? g_logp, Tensor? g_entropy, float temperature) -> Tensor",
+           lambda logits, *_: logits.new_empty(logits.shape))
+def token_logprobs_bwd(logits, target, stats, entropy, g_logp, g_entropy, temperature):
+    z, rows, inner, so, si = row_layout(logits)
+    vocab, dev = logits.shape[-1], logits.device
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if rows:
+        tgt = target.contiguous()
+        gl = g_logp.contiguous() if g_logp is not None else None
+        ge = g_entropy.contiguous() if g_entropy is not None else None
+        _lib.call_on(dev, "qb_token_logprobs_bwd", z.data_ptr(), _lib.tag(z.dtype), rows, inner,
+                     so, si, vocab, tgt.data_ptr(), temperature, stats.data_ptr(),
+                     _lib.ptr(entropy), _lib.ptr(gl), _lib.ptr(ge), out.data_ptr(),
+                     work=(rows * (2 * vocab * z.element_size() + 28), 0))
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# preference loss
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, mask, *args):
+        with _below_autograd():
+            loss, state = preference(logp, mask, *args)
+        ctx.save_for_backward(mask, state)
+        ctx.shape, ctx.dtype, ctx.args = logp.shape, logp.dtype, len(args)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(state)
+        return loss, state
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _g_state):
+        mask, state = ctx.saved_tensors
+        none = (None,) * (ctx.args + 1)
+        if g is None:
+            return None, *none
+        return preference_bwd(mask, state, g, *ctx.shape, ctx.dtype), *none
+
+
+def preference_state(n, cols):
+    """Floats of the op's second output: rewards [n], coefficients [n], then (16-byte aligned)
+    the kernels' workspace; and the workspace's offset."""
+    at = (2 * n + 3) // 4 * 4
+    return at + _lib.load().qb_preference_workspace(n // 2, cols) // 4, at
+
+
+def _preference_fake(logp, *_):
+    # the workspace's size is the library's to say; what is read of the state are its first 2n
+    n, cols = logp.shape
+    return logp.new_empty((), dtype=F32), logp.new_empty(
+        ((2 * n + 3) // 4 * 4 + n * ((cols + 2047) // 2048) * 4,), dtype=F32)
+
+
+@_register("preference(Tensor logp, Tensor? mask, Tensor? ref, Tensor? ref_row, "
+           "Tensor? denominator, float beta, float label_smoothing, float margin, "
+           "float divide_by, int loss_type, bool length_normalized) -> (Tensor, Tensor)",
+           _preference_fake, _Preference)
+def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, margin, divide_by,
+               loss_type, length_normalized):
+    n, cols = logp.shape
+    dev = logp.device
+    loss = torch.empty((), dtype=F32, device=dev)
+    size, at = preference_state(n, cols)
+    state = torch.empty(size, dtype=F32, device=dev)
+    base = state.data_ptr()
+    cfg = PreferenceConfig(beta, label_smoothing, margin, divide_by, loss_type,
+                           length_normalized)
+    e = logp.element_size()
+    _lib.call_on(dev, "qb_preference_fwd", logp.data_ptr(), _lib.ptr(ref), _lib.tag(logp.dtype),
+                 _lib.ptr(mask), _lib.ptr(ref_row), n // 2, cols, ctypes.addressof(cfg),
+                 _lib.ptr(denominator), loss.data_ptr(), base, base + 4 * n, base + 4 * at,
+                 kernels=2,
+                 work=(n * cols * (e * (1 if ref is None else 2) + (mask is not None)), 0))
+    return loss, state
+
+
+@_register("preference_bwd(Tensor? mask, Tensor state, Tensor g, SymInt n, SymInt cols, "
+           "ScalarType dtype) -> Tensor",
+           lambda mask, state, g, n, cols, dtype: state.new_empty((n, cols), dtype=dtype))
+def preference_bwd(mask, state, g, n, cols, dtype):
+    out = torch.empty((n, cols), dtype=dtype, device=state.device)
+    _lib.call_on(state.device, "qb_preference_bwd", _lib.ptr(mask), state.data_ptr() + 4 * n,
+                 g.data_ptr(), n // 2, cols, out.data_ptr(), _lib.tag(dtype),
+                 work=(n * cols * (out.element_size() + (mask is not None)), 0))
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# clipped policy loss
+
+
+class _Policy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, *args):
+        with _below_autograd():
+            loss, state, unit = policy(logp, *args)
+        ctx.save_for_backward(state, unit)
+        ctx.dtype, ctx.args, ctx.sequence, ctx.with_grad = logp.dtype, len(args), *args[-2:]
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(state, unit)
+        return loss, state, unit
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _g_state, _g_unit):
+        state, unit = ctx.saved_tensors
+        none = (None,) * ctx.args
+        if g is None:
+            return None, *none
+        if not ctx.with_grad:
+            raise RuntimeError("qlora_b200::policy: backward through a call made without the "
+                               "gradient (with_grad=False)")
+        return policy_bwd(unit, state, g, ctx.sequence, ctx.dtype), *none
+
+
+def policy_state(n, cols, sequence):
+    """Floats of the op's second output: statistics [4], weights (one, or [n]), then (16-byte
+    aligned) the kernels' workspace; and the workspace's offset."""
+    at = (4 + (n if sequence else 1) + 3) // 4 * 4
+    return at + _lib.load().qb_policy_workspace(n, cols) // 4, at
+
+
+def _policy_fake(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_high, delta,
+                 kl_coef, divide_by, sequence, with_grad):
+    n, cols = logp.shape
+    at = (4 + (n if sequence else 1) + 3) // 4 * 4
+    return (logp.new_empty((), dtype=F32),
+            logp.new_empty((at + n * ((cols + 2047) // 2048) * 8,), dtype=F32),
+            logp.new_empty((n if with_grad else 0, cols), dtype=F32))
+
+
+@_register("policy(Tensor logp, Tensor? old_logp, Tensor advantages, Tensor? mask, Tensor? ref, "
+           "Tensor? denominator, float clip_low, float clip_high, float delta, float kl_coef, "
+           "float divide_by, bool sequence, bool with_grad) -> (Tensor, Tensor, Tensor)",
+           _policy_fake, _Policy)
+def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_high, delta,
+           kl_coef, divide_by, sequence, with_grad):
+    n, cols = logp.shape
+    dev = logp.device
+    loss = torch.empty((), dtype=F32, device=dev)
+    size, at = policy_state(n, cols, sequence)
+    state = torch.empty(size, dtype=F32, device=dev)
+    base = state.data_ptr()
+    unit = torch.empty((n if with_grad else 0, cols), dtype=F32, device=dev)
+    cfg = PolicyConfig(clip_low, clip_high, delta, kl_coef, divide_by, sequence, 0)
+    per_token = advantages.dim() == 2
+    arrays = 1 + (old_logp is not None) + (ref is not None)
+    _lib.call_on(dev, "qb_policy_fwd", logp.data_ptr(), _lib.ptr(old_logp), _lib.ptr(ref),
+                 _lib.tag(logp.dtype), advantages.data_ptr(), advantages.stride(0),
+                 advantages.stride(1) if per_token else 0, _lib.ptr(mask), n, cols,
+                 ctypes.addressof(cfg), _lib.ptr(denominator), loss.data_ptr(), base, base + 16,
+                 unit.data_ptr() if with_grad else None, base + 4 * at, kernels=2,
+                 work=(n * cols * (arrays * logp.element_size() + 4 * per_token + 4 * with_grad
+                                   + (mask is not None)), 0))
+    return loss, state, unit
+
+
+@_register("policy_bwd(Tensor unit, Tensor state, Tensor g, bool sequence, ScalarType dtype) "
+           "-> Tensor",
+           lambda unit, state, g, sequence, dtype: unit.new_empty(unit.shape, dtype=dtype))
+def policy_bwd(unit, state, g, sequence, dtype):
+    n, cols = unit.shape
+    out = torch.empty((n, cols), dtype=dtype, device=unit.device)
+    _lib.call_on(unit.device, "qb_policy_bwd", unit.data_ptr(), state.data_ptr() + 16,
+                 int(sequence), g.data_ptr(), n, cols, out.data_ptr(), _lib.tag(dtype),
+                 work=(n * cols * (4 + out.element_size()), 0))
+    return out
+
+
+def ops():
+    """Every op of this module (for checks such as torch.library.opcheck)."""
+    return {name: getattr(torch.ops.qlora_b200, name) for name in (
+        "token_logprobs", "token_logprobs_bwd", "preference", "preference_bwd", "policy",
+        "policy_bwd")}
+
+
+# ------------------------------------------------------------------------------------------
+# argument checks the objectives share
+
+
+def constant(what, name, t, logp):
+    """`t` as a constant of an objective over `logp`: on its device, no part of a graph."""
+    if t.device != logp.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, logp on {logp.device}")
+    if t.requires_grad:
+        raise ValueError(f"{what}: {name} is a constant of the objective (no gradient flows into "
+                         "it); pass it detached")
+    return t
+
+
+def mask_bytes(what, mask, logp):
+    """The mask as contiguous bytes (nonzero: the token counts), or None."""
+    if mask is None:
+        return None
+    if mask.shape != logp.shape or mask.device != logp.device:
+        raise ValueError(f"{what}: mask {tuple(mask.shape)} on {mask.device} for logp "
+                         f"{tuple(logp.shape)} on {logp.device}")
+    if mask.dtype not in (torch.bool, torch.uint8):
+        mask = mask != 0
+    return mask.contiguous()
+
+
+def divisor(what, denominator, device):
+    """(device double or None, number or 0.0) of a denominator given as a tensor, a number or
+    None. A tensor is not read on the host."""
+    if denominator is None:
+        return None, 0.0
+    if torch.is_tensor(denominator):
+        if denominator.numel() != 1:
+            raise ValueError(f"{what}: the denominator is one number")
+        return denominator.detach().reshape(()).to(device=device, dtype=torch.float64), 0.0
+    value = float(denominator)
+    if not 0.0 < value < float("inf"):
+        raise ValueError(f"{what}: denominator {denominator} is not positive")
+    return None, value
+
+
+def logp_matrix(what, logp):
+    """logp as the objectives read it: a CUDA [rows, tokens] matrix of a kernel dtype."""
+    _lib.require_cuda(logp, what=what)
+    if logp.dim() != 2 or logp.shape[0] == 0 or logp.shape[1] == 0:
+        raise ValueError(f"{what}: logp is [rows, tokens], got {tuple(logp.shape)}")
+    _lib.tag(logp.dtype)
+    return logp

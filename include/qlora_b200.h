@@ -447,6 +447,116 @@ int qb_monitor_report(int device, char* buf, int64_t len);
  * QB_ERR_TIMEOUT and the context stays usable. */
 int qb_selftest_bounded_wait(int64_t limit_ns, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Post-training objectives and gradient clipping (no counterpart in the reference)
+ */
+
+/* Per row of logits: logp = (z[label] - m) / T - ln sum exp((z - m) / T) with m the row's maximum
+ * (0 for labels outside [0, vocab)), and, when `entropy` is given, the entropy of the row's
+ * distribution. Row r of `rows` starts at (r / inner) * stride_outer + (r % inner) *
+ * stride_inner elements, so a [batch, positions, vocab] view needs no copy; the last dimension
+ * is contiguous. stats [rows, 2] (8-byte aligned) receives (m, sum) for the backward. Logits of
+ * -inf have probability 0; a row of nothing else is NaN. T in 1e-6 .. 1e6. */
+int qb_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t inner,
+                      int64_t stride_outer, int64_t stride_inner, int64_t vocab,
+                      const int64_t* target, float temperature, float* logp, float* entropy,
+                      float* stats, cudaStream_t stream);
+
+/* dlogits [rows, vocab] (contiguous, the logits' dtype) of the sum of g_logp * logp + g_entropy *
+ * entropy: (g (onehot - p) - g_entropy p (ln p + entropy)) / T. g_logp or g_entropy may be NULL
+ * (zeros); `entropy` is the forward's, needed with g_entropy. A row whose gradients are zero is
+ * written as zeros without being read. */
+int qb_token_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t inner,
+                          int64_t stride_outer, int64_t stride_inner, int64_t vocab,
+                          const int64_t* target, float temperature, const float* stats,
+                          const float* entropy, const float* g_logp, const float* g_entropy,
+                          void* dlogits, cudaStream_t stream);
+
+/* loss_type 0 sigmoid, 1 hinge, 2 ipo; denominator 0: the number of pairs. */
+typedef struct qb_preference_config {
+  double beta, label_smoothing, margin, denominator;
+  int32_t loss_type, length_normalized;
+} qb_preference_config;
+
+/* sizeof(qb_preference_config): the layout check of a binding that builds the struct itself. */
+int64_t qb_preference_config_size(void);
+
+/* Bytes of workspace qb_preference_fwd needs (0: bad shape). */
+int64_t qb_preference_workspace(int64_t pairs, int64_t cols);
+
+/* Preference loss over logp [2 * pairs, cols] (contiguous; the first half the preferred sequences,
+ * the second half the rejected ones, pair by pair): with s = sum mask (logp - ref) of a sequence
+ * (divided by its unmasked count when length_normalized, minus ref_row), D = s_preferred -
+ * s_rejected and u = beta D - margin, the sum over the pairs of
+ *   sigmoid  -(1 - label_smoothing) ln sigma(u) - label_smoothing ln sigma(-u)
+ *   hinge    max(0, 1 - u)                     ipo  (D - 1 / (2 beta))^2
+ * over the denominator (*denominator, a device double, when given). ref [2 * pairs, cols] in
+ * logp's dtype, or ref_row [2 * pairs], or neither; mask bytes [2 * pairs, cols] or NULL (all).
+ * rewards [2 * pairs] = beta s; coef [2 * pairs] is what qb_preference_bwd takes. `cfg` is a host
+ * pointer; workspace is 16-byte aligned device memory. */
+int qb_preference_fwd(const void* logp, const void* ref, int dtype, const uint8_t* mask,
+                      const float* ref_row, int64_t pairs, int64_t cols,
+                      const qb_preference_config* cfg, const double* denominator, float* loss,
+                      float* rewards, float* coef, void* workspace, cudaStream_t stream);
+
+/* grad [2 * pairs, cols] = mask * coef[row] * *g in `dtype` (g: the loss's gradient, a device
+ * float). */
+int qb_preference_bwd(const uint8_t* mask, const float* coef, const float* g, int64_t pairs,
+                      int64_t cols, void* grad, int dtype, cudaStream_t stream);
+
+/* delta 0: none (otherwise above 1 + clip_high); reduction 0 token, 1 sequence; denominator 0: the
+ * unmasked tokens (token) or the rows (sequence). */
+typedef struct qb_policy_config {
+  double clip_low, clip_high, delta, kl_coef, denominator;
+  int32_t reduction, pad;
+} qb_policy_config;
+
+/* sizeof(qb_policy_config): the layout check of a binding that builds the struct itself. */
+int64_t qb_policy_config_size(void);
+
+/* Bytes of workspace qb_policy_fwd needs (0: bad shape). */
+int64_t qb_policy_workspace(int64_t rows, int64_t cols);
+
+/* Clipped policy loss over logp [rows, cols] (contiguous): with r = exp(logp - old_logp) and
+ * d = ref - logp, per unmasked token
+ *   -min(min(r, delta) A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)
+ * summed over all tokens (token), or averaged over each row's unmasked tokens and summed over the
+ * rows (sequence), over the denominator (*denominator, a device double, when given). old_logp
+ * NULL: r = 1 (the policy itself); ref NULL: no KL term; both in logp's dtype. advantages are
+ * read at row * adv_row_stride + col * adv_col_stride (a stride of 0 broadcasts). mask bytes
+ * [rows, cols] or NULL (all).
+ * stats [4]: unmasked tokens, the mean of exp(d) - d - 1, the shares of the tokens whose gradient
+ * the lower and the upper border hold. weight ([1] for token, [rows] for sequence) and unit_grad
+ * ([rows, cols] fp32, each token's dL/dlogp before the reduction; NULL when no gradient follows)
+ * are what qb_policy_bwd takes. `cfg` is a host pointer; workspace is 16-byte aligned. */
+int qb_policy_fwd(const void* logp, const void* old_logp, const void* ref, int dtype,
+                  const float* advantages, int64_t adv_row_stride, int64_t adv_col_stride,
+                  const uint8_t* mask, int64_t rows, int64_t cols, const qb_policy_config* cfg,
+                  const double* denominator, float* loss, float* stats, float* weight,
+                  float* unit_grad, void* workspace, cudaStream_t stream);
+
+/* grad [rows, cols] = unit_grad * weight[row * weight_row_stride] * *g in `dtype`. */
+int qb_policy_bwd(const float* unit_grad, const float* weight, int64_t weight_row_stride,
+                  const float* g, int64_t rows, int64_t cols, void* grad, int dtype,
+                  cudaStream_t stream);
+
+/* Doubles of workspace qb_grad_norm and qb_grad_clip need for n_tensors tensors. */
+int64_t qb_grad_norm_workspace(int64_t n_tensors);
+
+/* norm[0] = the norm of all elements of n_tensors contiguous tensors together, of order 1, 2 or 0
+ * (infinity), from 64-bit sums in a fixed order; 0 without elements, NaN when one is. ptrs (device
+ * addresses), sizes (elements) and dtypes (QB_F32, QB_F16, QB_BF16, each tensor its own) are
+ * host arrays, read before the call returns. */
+int qb_grad_norm(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* dtypes,
+                 int64_t n_tensors, int order, double* workspace, int64_t workspace_doubles,
+                 float* norm, cudaStream_t stream);
+
+/* qb_grad_norm, then every element times min(1, *max_norm / (norm + 1e-6)), in place (nothing is
+ * written when that is 1). max_norm is a host pointer. Tensors that share memory are refused. */
+int qb_grad_clip(const uint64_t* ptrs, const int64_t* sizes, const uint8_t* dtypes,
+                 int64_t n_tensors, int order, const double* max_norm, double* workspace,
+                 int64_t workspace_doubles, float* norm, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
