@@ -108,6 +108,7 @@ def test_row_layout_reads_views_in_place():
 
 def test_c_entries_refuse_before_any_launch():
     fake = 1 << 20
+    keep = []
 
     def lp(rows=4, inner=1, vocab=10, t=1.0, dtype=0, logits=fake, out=fake):
         return ("qb_token_logprobs", logits, dtype, rows, inner, vocab, 0, vocab, fake, t, out,
@@ -124,6 +125,7 @@ def test_c_entries_refuse_before_any_launch():
     pref = oo.PreferenceConfig(0.1, 0.0, 0.0, 0.0, 0, 0)
 
     def pr(cfg=pref, pairs=2, cols=8, ref=None, row=None, logp=fake, **kw):
+        keep.append(cfg)               # the call reads it at its address
         at = ctypes.addressof(cfg) if cfg is not None else None
         return ("qb_preference_fwd", logp, ref, 0, None, row, pairs, cols, at, None, fake, fake,
                 fake, fake, None)
@@ -138,6 +140,7 @@ def test_c_entries_refuse_before_any_launch():
     cases.append((("qb_preference_bwd", None, None, fake, 2, 8, fake, 0, None), "null"))
 
     def po(cfg, rows=2, cols=8, adv=fake):
+        keep.append(cfg)
         return ("qb_policy_fwd", fake, fake, None, 0, adv, 1, 0, None, rows, cols,
                 ctypes.addressof(cfg), None, fake, fake, fake, fake, fake, None)
 
@@ -160,7 +163,6 @@ def test_c_entries_refuse_before_any_launch():
         return ("qb_grad_clip", *table(ptrs, sizes, tags), order, ctypes.addressof(keep[-1]),
                 fake, 1 << 20, fake, None)
 
-    keep = []
     cases += [(("qb_grad_norm", None, None, None, 1, 2, fake, 99, fake, None), "null"),
               (("qb_grad_norm", *table([fake], [4], [0]), 2, fake, 0, fake, None), "too small"),
               (("qb_grad_norm", *table([fake], [4], [0]), 3, fake, 99, fake, None), "order"),
