@@ -16,9 +16,13 @@ from dataclasses import dataclass, replace
 import torch
 import torch.nn.functional as F
 
-from .cross_entropy import fused_causal_lm_loss
+from .cross_entropy import IGNORE_INDEX, fused_causal_lm_loss, shift_labels_of
+from .grad_norm import clip_grad_norm_
+from .logprobs import linear_token_logprobs
 from .lora import DropoutCast, ScaledAdd
 from .nf4 import NF4Linear, quantize_nf4
+from .policy import policy_loss
+from .preference import preference_loss
 from .rmsnorm import rmsnorm
 from .rope import CudaRoPE
 from .swiglu import swiglu
@@ -645,6 +649,20 @@ class QwenQLoRA(torch.nn.Module):
         return self._rope[key]
 
     def forward(self, input_ids, labels, num_items_in_batch=None):
+        h = self.hidden_states(input_ids)
+        return fused_causal_lm_loss(h, self.lm_head, labels, num_items_in_batch=num_items_in_batch)
+
+    def token_logprobs(self, input_ids, labels):
+        """(logp, entropy, mask), each [B, S]: at position t the log-probability of the label at
+        t + 1 (labels shifted as in the loss; 0 where it is -100, and in the last position), the
+        entropy of that prediction, and which positions are scored. The log-probabilities are
+        differentiable in the adapters."""
+        target = shift_labels_of(labels)
+        logp, entropy = linear_token_logprobs(self.hidden_states(input_ids), self.lm_head, target)
+        return logp, entropy, target != IGNORE_INDEX
+
+    def hidden_states(self, input_ids):
+        """The final norm's output [B, S, hidden]."""
         B, S = input_ids.shape
         dev = input_ids.device
         if MASKS and dev in _SIDE_STREAMS:   # masks a side stream may still be writing
@@ -690,8 +708,7 @@ class QwenQLoRA(torch.nn.Module):
                                                       determinism_check="none")
             else:
                 h = layer(h, cos, sin, seeds[i], None, prefetcher(i + 1), mask_jobs(i))
-        h = rmsnorm(h, self.norm, self.shape.eps)
-        return fused_causal_lm_loss(h, self.lm_head, labels, num_items_in_batch=num_items_in_batch)
+        return rmsnorm(h, self.norm, self.shape.eps)
 
     def layer_seed(self, i):
         """Per (step, layer) dropout seed; projection k of the layer draws with seed + k."""
@@ -717,16 +734,54 @@ def make_optimizer(model, lr=1e-4):
                              weight_decay=0.0, fused=True)
 
 
-def train_step(model, opt, input_ids, labels, grad_sync=None, num_items_in_batch=None):
-    """One optimizer step; returns the loss tensor (on the device, not synchronised)."""
-    model.train()
-    loss, _ = model(input_ids, labels, num_items_in_batch=num_items_in_batch)
+def _update(model, opt, loss, grad_sync, max_grad_norm):
+    """Backward, gradient sync, clipping (over all ranks' summed gradients) and optimizer step."""
     loss.backward()
     if grad_sync is not None:
         grad_sync()
+    if max_grad_norm is not None:
+        clip_grad_norm_(model.adapter_parameters(), max_grad_norm)
     opt.step()
     # with a gradient sync the .grad tensors are views into its flat buffer and stay; without
     # one, dropping them lets the next backward hand its fresh gradients over without an add
     opt.zero_grad(set_to_none=grad_sync is None)
     model.step_seed += 1
     return loss.detach()
+
+
+def train_step(model, opt, input_ids, labels, grad_sync=None, num_items_in_batch=None,
+               max_grad_norm=None):
+    """One optimizer step on the next-token loss; returns the loss tensor (on the device, not
+    synchronised). max_grad_norm: the adapters' gradients are scaled to that norm first when
+    theirs is larger."""
+    model.train()
+    loss, _ = model(input_ids, labels, num_items_in_batch=num_items_in_batch)
+    return _update(model, opt, loss, grad_sync, max_grad_norm)
+
+
+def preference_step(model, opt, input_ids, labels, ref_logp=None, grad_sync=None,
+                    max_grad_norm=None, **objective):
+    """One optimizer step on the preference loss; returns it and the PreferenceStep (both on the
+    device, not synchronised). input_ids / labels [2P, S]: the preferred sequences, then the
+    rejected ones, labels -100 where a token is not part of the answer. ref_logp: the reference's
+    log-probabilities as preference_loss takes them (per token as model.token_logprobs lays them
+    out, or per sequence). objective: preference_loss's other arguments; under data parallelism
+    its denominator is the global number of pairs."""
+    model.train()
+    logp, _, mask = model.token_logprobs(input_ids, labels)
+    loss, step = preference_loss(logp, mask, ref_logp, **objective)
+    return _update(model, opt, loss, grad_sync, max_grad_norm), step
+
+
+def policy_step(model, opt, input_ids, labels, old_logp, advantages, ref_logp=None,
+                grad_sync=None, max_grad_norm=None, **objective):
+    """One optimizer step on the clipped policy loss of sampled sequences; returns it and the
+    PolicyStep (both on the device, not synchronised). labels are -100 where a token was not
+    sampled; old_logp and ref_logp [N, S] as model.token_logprobs lays them out, old_logp None
+    for the policy itself; advantages [N] or [N, S]. objective: policy_loss's other arguments;
+    under data parallelism its denominator is the global number of scored tokens (token) or of
+    sequences (sequence)."""
+    model.train()
+    logp, _, mask = model.token_logprobs(input_ids, labels)
+    loss, step = policy_loss(logp, old_logp, advantages, mask, ref_logp, **objective)
+    return _update(model, opt, loss, grad_sync, max_grad_norm), step
