@@ -2,19 +2,21 @@
 // materialised logits, forward and backward.
 //
 // With temperature T, c = log2(e) / T and a row's maximum m:
-//   y_j = (z_j - m) c,  e_j = 2^y_j,  s = sum e_j,  t = sum e_j y_j
-//   logp = (z_label - m) / T - ln s          H = ln s - ln2 t / s
+//   d_j = z_j - m,  e_j = 2^(c d_j),  s = sum e_j,  t = sum e_j d_j
+//   logp = d_label / T - ln s                H = ln s - t / (s T)
 //   dz_j = (1/T) [ g (1{j = label} - p_j) - g_H p_j (ln p_j + H) ],  p_j = e_j / s
-//        = e_j (A + B y_j) + (g / T) 1{j = label}
-//   with A = -(g + g_H (H - ln s)) / (T s),  B = -g_H ln2 / (T s)
+//        = e_j (A + B d_j) + (g / T) 1{j = label}
+//   with A = -(g + g_H (H - ln s)) / (T s),  B = -g_H / (T^2 s)
 // Sums and maxima are fp32. The maximum is subtracted before the scale: z c - m c in one fused
-// multiply-add would save an operation, but leaves the rounding of m c in every y, which grows with
-// |m| / T, and makes a certain token's log-probability something near 0 instead of 0.
+// multiply-add would save an operation, but leaves the rounding of m c in every exponent, which
+// grows with |m| / T, and makes a certain token's log-probability something near 0 instead of 0.
 //
-// A banned token (a logit of -inf, or so low that y is) has e = 0 and no e y term: y is held above
-// kLowest, where 2^y is 0 and y stays finite. Rows need no other care: one of equal lowest values
-// is the uniform distribution, one of -inf alone, with +inf or with NaN is NaN, as the formula is.
+// A banned token (a logit of -inf) has e = 0 and no e d term: d is held at -300 T, where e is 0 and
+// every product with d finite. Rows need no other care: one of equal lowest values is the uniform distribution, one of -inf
+// alone, with +inf or with NaN is NaN, as the formula is.
 #include <cooperative_groups.h>
+
+#include <cstring>
 
 #include "qb_common.cuh"
 
@@ -23,9 +25,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 512;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-constexpr float kLowest = -1e5f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float y) {
   float r;
@@ -47,28 +47,111 @@ struct Rows {
   }
 };
 
-// max, sum 2^(y), sum 2^(y) y of a set of elements, y relative to m.
+// ---------------------------------------------------------------------------------------------
+// Two fp32 values in one 64-bit register: one issue slot for two additions or multiplications.
+
+using Pair = unsigned long long;
+
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves(Pair p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 16 bytes of logits as pairs of fp32 values, and their maximum (a NaN stays one).
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  uint4 u;
+  __device__ __forceinline__ Pair at(int k) const {
+    return k == 0 ? pair(__uint_as_float(u.x), __uint_as_float(u.y))
+                  : pair(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  __device__ __forceinline__ float top() const {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
+                   max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  static __device__ __forceinline__ uint32_t none() { return 0xff800000u; }   // -inf
+};
+template <typename H2>
+__device__ __forceinline__ H2 word_as(uint32_t w) {
+  H2 h;
+  memcpy(&h, &w, 4);
+  return h;
+}
+template <typename T, typename H2> struct Vec16Bit {
+  static constexpr int N = 8;
+  uint4 u;
+  __device__ __forceinline__ uint32_t word(int k) const {
+    return k == 0 ? u.x : k == 1 ? u.y : k == 2 ? u.z : u.w;
+  }
+  __device__ __forceinline__ float top() const {
+    const H2 m = __hmax2_nan(__hmax2_nan(word_as<H2>(u.x), word_as<H2>(u.y)),
+                             __hmax2_nan(word_as<H2>(u.z), word_as<H2>(u.w)));
+    return max_nan(qb::to_f(m.x), qb::to_f(m.y));
+  }
+};
+template <> struct Vec<__nv_bfloat16> : Vec16Bit<__nv_bfloat16, __nv_bfloat162> {
+  __device__ __forceinline__ Pair at(int k) const {
+    const uint32_t w = word(k);
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t none() { return 0xff80ff80u; }
+};
+template <> struct Vec<__half> : Vec16Bit<__half, __half2> {
+  __device__ __forceinline__ Pair at(int k) const {
+    const float2 f = __half22float2(word_as<__half2>(word(k)));
+    return pair(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint32_t none() { return 0xfc00fc00u; }
+};
+
+// max, sum 2^(d c), sum 2^(d c) d of a set of elements, d relative to m.
 struct Stat {
   float m, s, t;
 };
 
+// c, and the d below which nothing is left of e.
+struct Scale {
+  float c, low;
+  __device__ __forceinline__ explicit Scale(float inv_t) : c(inv_t * kLog2e), low(-300.f / inv_t) {}
+};
+
 // From one maximum to a larger one (from -inf, with s = t = 0, too).
-__device__ __forceinline__ void rescale(Stat& a, float m, float c) {
-  const float d = fmaxf((a.m - m) * c, kLowest);
-  const float f = ex2(d);
+__device__ __forceinline__ void rescale(Stat& a, float m, Scale c) {
+  const float d = fmaxf(a.m - m, c.low);
+  const float f = ex2(d * c.c);
   a.t = (a.t + a.s * d) * f;
   a.s *= f;
   a.m = m;
 }
 
-__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
+__device__ __forceinline__ Stat merge(Stat a, Stat b, Scale c) {
   const float m = fmaxf(a.m, b.m);
   rescale(a, m, c);
   rescale(b, m, c);
   return {m, a.s + b.s, a.t + b.t};
 }
 
-__device__ __forceinline__ Stat warp_merge(Stat st, float c) {
+__device__ __forceinline__ Stat warp_merge(Stat st, Scale c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Stat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
@@ -78,21 +161,46 @@ __device__ __forceinline__ Stat warp_merge(Stat st, float c) {
   return st;
 }
 
-template <typename T, bool ENT>
-__device__ __forceinline__ void add(Stat& st, const float* z, int n, float c) {
-  float m = z[0];
+// U vectors of a thread: one maximum and at most one rescaling for all of them.
+template <typename T, bool ENT, int U>
+__device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scale c) {
+  float m = x[0].top();
 #pragma unroll
-  for (int e = 1; e < n; ++e) m = max_nan(m, z[e]);
+  for (int u = 1; u < U; ++u) m = max_nan(m, x[u].top());
   if (m == -INFINITY) return;    // all banned: nothing to add, and no maximum to subtract
   if (m > st.m) rescale(st, m, c);
+  const Pair minus = pair(-st.m, -st.m), cc = pair(c.c, c.c);
+  Pair s = pair(st.s, 0.f), t = pair(st.t, 0.f);
 #pragma unroll
-  for (int e = 0; e < n; ++e) {
-    float y = (z[e] - st.m) * c;
-    if (ENT) y = max_nan(y, kLowest);
-    const float x = ex2(y);
-    st.s += x;
-    if (ENT) st.t += x * y;
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int k = 0; k < Vec<T>::N / 2; ++k) {
+      Pair d = add2(x[u].at(k), minus);
+      float lo, hi;
+      halves(mul2(d, cc), lo, hi);
+      const Pair e = pair(ex2(lo), ex2(hi));
+      s = add2(s, e);
+      if (ENT) {
+        halves(d, lo, hi);
+        t = fma2(e, pair(max_nan(lo, c.low), max_nan(hi, c.low)), t);
+      }
+    }
   }
+  float lo, hi;
+  halves(s, lo, hi);
+  st.s = lo + hi;
+  halves(t, lo, hi);
+  st.t = lo + hi;
+}
+
+template <bool ENT>
+__device__ __forceinline__ void add_one(Stat& st, float z, Scale c) {
+  if (z == -INFINITY) return;
+  if (z > st.m) rescale(st, z, c);
+  const float d = max_nan(z - st.m, c.low);
+  const float e = ex2(d * c.c);
+  st.s += e;
+  if (ENT) st.t += e * d;
 }
 
 // One CTA per row, or a cluster of CTAs when there are few rows: each takes every CS-th vector
@@ -103,7 +211,7 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
                       const int64_t* __restrict__ target, float inv_t,
                       float* __restrict__ logp, float* __restrict__ entropy,
                       float2* __restrict__ stats) {
-  constexpr int VE = 16 / sizeof(T);
+  constexpr int VE = Vec<T>::N;
   constexpr int U = 4;
   __shared__ Stat warp_stat[32];
   __shared__ Stat cta_stat;
@@ -112,7 +220,7 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
   const int rank = static_cast<int>(cluster.block_rank());
   const int64_t row = blockIdx.x / cs;
   const T* z = logits + rows.offset(row);
-  const float c = inv_t * kLog2e;
+  const Scale c(inv_t);
   const int tid = rank * kThreads + threadIdx.x, nthreads = cs * kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
@@ -143,27 +251,24 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
   };
 
   Stat st{-INFINITY, 0.f, 0.f};
-  for (int v = tid; v < nvec; v += U * nthreads) {
-    qb::Vec16<T> x[U];
+  const uint4 none = {Vec<T>::none(), Vec<T>::none(), Vec<T>::none(), Vec<T>::none()};
+  auto load = [&](Vec<T>(&x)[U], int v) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v + u * nthreads < nvec)
-        x[u].u = __ldg(reinterpret_cast<const uint4*>(body + int64_t(v + u * nthreads) * VE));
+      x[u].u = v + u * nthreads < nvec
+                   ? __ldg(reinterpret_cast<const uint4*>(body + int64_t(v + u * nthreads) * VE))
+                   : none;
+  };
+  Vec<T> x[U], next[U];
+  load(x, tid);
+  for (int v = tid; v < nvec; v += U * nthreads) {
+    load(next, v + U * nthreads);      // in flight while this batch is added up
+    add_vectors<T, ENT, U>(st, x, c);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v + u * nthreads < nvec) {
-        float f[VE];
-#pragma unroll
-        for (int e = 0; e < VE; ++e) f[e] = qb::to_f(x[u].v[e]);
-        add<T, ENT>(st, f, VE, c);
-      }
-    }
+    for (int u = 0; u < U; ++u) x[u] = next[u];
   }
-  for (int j = tid; j < vocab - nvec * VE; j += nthreads) {
-    const int col = j < head ? j : nvec * VE + j;
-    const float f = qb::to_f(z[col]);
-    add<T, ENT>(st, &f, 1, c);
-  }
+  for (int j = tid; j < vocab - nvec * VE; j += nthreads)
+    add_one<ENT>(st, qb::to_f(z[j < head ? j : nvec * VE + j]), c);
   st = cluster_merge(st);
   if (rank == 0 && threadIdx.x == 0) {
     const int64_t label = target[row];
@@ -171,7 +276,7 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
     float lp = 0.f;
     if (label >= 0 && label < vocab) lp = (qb::to_f(z[label]) - st.m) * inv_t - log_s;
     logp[row] = lp;
-    if (ENT) entropy[row] = log_s - kLn2 * (st.t / st.s);
+    if (ENT) entropy[row] = log_s - inv_t * (st.t / st.s);
     stats[row] = make_float2(st.m, st.s);
   }
 }
@@ -180,6 +285,55 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
 // backward: elementwise given the row's (m, s, H); one CTA per (row, tile of columns)
 
 constexpr int kBwdThreads = 256;
+constexpr int kBwdVectors = 8;         // per thread and tile: 32 KB of logits a CTA
+
+__device__ __forceinline__ uint32_t packed(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &h, 4);
+  return w;
+}
+__device__ __forceinline__ uint32_t packed(float lo, float hi, __half) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &h, 4);
+  return w;
+}
+
+// The row's numbers, and dlogits of one element or one vector without the target's term.
+struct RowGrad {
+  float m, a, b;
+  Scale c;
+  __device__ __forceinline__ float one(float z) const {
+    const float d = max_nan(z - m, c.low);
+    return ex2(d * c.c) * fmaf(b, d, a);
+  }
+  __device__ __forceinline__ void two(Pair z, float& lo, float& hi) const {
+    float x, y;
+    halves(add2(z, pair(-m, -m)), x, y);
+    const Pair d = pair(max_nan(x, c.low), max_nan(y, c.low));
+    halves(mul2(d, pair(c.c, c.c)), x, y);
+    halves(mul2(pair(ex2(x), ex2(y)), fma2(pair(b, b), d, pair(a, a))), lo, hi);
+  }
+  __device__ __forceinline__ uint4 vec(const Vec<float>& x) const {
+    float f[4];
+    two(x.at(0), f[0], f[1]);
+    two(x.at(1), f[2], f[3]);
+    return {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+            __float_as_uint(f[3])};
+  }
+  template <typename T>
+  __device__ __forceinline__ uint4 vec(const Vec<T>& x) const {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float lo, hi;
+      two(x.at(k), lo, hi);
+      w[k] = packed(lo, hi, T());
+    }
+    return {w[0], w[1], w[2], w[3]};
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kBwdThreads)
@@ -188,8 +342,8 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
                           const float2* __restrict__ stats, const float* __restrict__ entropy,
                           const float* __restrict__ g_logp, const float* __restrict__ g_ent,
                           T* __restrict__ dlogits) {
-  constexpr int VE = 16 / sizeof(T);
-  constexpr int U = 4;
+  constexpr int VE = Vec<T>::N;
+  constexpr int U = kBwdVectors;
   const int64_t row = blockIdx.x / tiles;
   const int tile = blockIdx.x % tiles;
   const T* z = logits + rows.offset(row);
@@ -198,50 +352,61 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
   const bool labelled = label >= 0 && label < vocab;
   const float g = labelled && g_logp ? g_logp[row] : 0.f;
   const float gh = g_ent ? g_ent[row] : 0.f;
-  const float2 ms = stats[row];
-  const float c = inv_t * kLog2e, k = inv_t / ms.y;
-  const float log_s = logf(ms.y);
-  const float A = -(g + (g_ent ? gh * (entropy[row] - log_s) : 0.f)) * k;
-  const float B = -gh * kLn2 * k;
-  const float hot = g * inv_t;
   const bool zero = g == 0.f && gh == 0.f;   // e.g. a prompt's positions: nothing to read
 
-  auto value = [&](float zf, int col) -> float {
-    if (zero) return 0.f;
-    const float y = max_nan((zf - ms.x) * c, kLowest);
-    const float x = ex2(y);
-    const float d = x * fmaf(B, y, A);
-    return col == label && labelled ? d + hot : d;
-  };
-
+  // scalars before the first 16-byte boundary of the gradient and after its last
   const int head = min(vocab, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dz) & 15)) & 15)
                                                / sizeof(T)));
   const int nvec = (vocab - head) / VE;
+  const int v0 = tile * (kBwdThreads * U) + threadIdx.x;
+  if (zero) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * kBwdThreads < nvec)
+        *reinterpret_cast<uint4*>(dz + head + int64_t(v0 + u * kBwdThreads) * VE) = {0, 0, 0, 0};
+    if (tile == 0)
+      for (int j = threadIdx.x; j < vocab - nvec * VE; j += kBwdThreads)
+        dz[j < head ? j : nvec * VE + j] = qb::from_f<T>(0.f);
+    return;
+  }
   const bool vec_in = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
-  const int v0 = tile * (kBwdThreads * U);
+  Vec<T> x[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int v = v0 + u * kBwdThreads + threadIdx.x;
+    const int v = v0 + u * kBwdThreads;
     if (v < nvec) {
-      const int col = head + v * VE;
-      float f[VE];
-      if (!zero) {
-        if (vec_in) {
-          qb::load16<T>(z + col, f);
-        } else {
+      const T* p = z + head + int64_t(v) * VE;
+      if (vec_in) {
+        x[u].u = __ldg(reinterpret_cast<const uint4*>(p));
+      } else {
+        T f[VE];
 #pragma unroll
-          for (int e = 0; e < VE; ++e) f[e] = qb::to_f(z[col + e]);
-        }
+        for (int e = 0; e < VE; ++e) f[e] = p[e];
+        memcpy(&x[u].u, f, 16);
       }
+    }
+  }
+  const float2 ms = stats[row];
+  const float k = inv_t / ms.y, log_s = logf(ms.y);
+  const float hot = g * inv_t;
+  const RowGrad grad{ms.x, -(g + (g_ent ? gh * (entropy[row] - log_s) : 0.f)) * k,
+                     -gh * inv_t * k, Scale(inv_t)};
+  // the target's element takes its term in the thread that writes it
+  const int hot_col = labelled ? static_cast<int>(label) : -1;
+  const int hot_vec = hot_col >= head && hot_col < head + nvec * VE ? (hot_col - head) / VE : -1;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = value(f[e], col + e);
-      qb::store16<T>(dz + col, f);
+  for (int u = 0; u < U; ++u) {
+    const int v = v0 + u * kBwdThreads;
+    if (v < nvec) {
+      const uint4 out = grad.vec(x[u]);
+      *reinterpret_cast<uint4*>(dz + head + int64_t(v) * VE) = out;
+      if (v == hot_vec) dz[hot_col] = qb::from_f<T>(grad.one(qb::to_f(z[hot_col])) + hot);
     }
   }
   if (tile == 0) {
     for (int j = threadIdx.x; j < vocab - nvec * VE; j += kBwdThreads) {
       const int col = j < head ? j : nvec * VE + j;
-      dz[col] = qb::from_f<T>(value(zero ? 0.f : qb::to_f(z[col]), col));
+      dz[col] = qb::from_f<T>(grad.one(qb::to_f(z[col])) + (col == hot_col ? hot : 0.f));
     }
   }
 }
@@ -309,7 +474,7 @@ extern "C" int qb_token_logprobs_bwd(const void* logits, int dtype, int64_t rows
     return qb::fail(QB_ERR_INVALID, "token_logprobs_bwd: null pointer");
   const Rows r{inner, stride_outer, stride_inner};
   QB_DISPATCH_FLOAT(dtype, T, {
-    constexpr int kTile = kBwdThreads * 4 * (16 / sizeof(T));
+    constexpr int kTile = kBwdThreads * kBwdVectors * (16 / sizeof(T));
     const int64_t tiles = (vocab + kTile - 1) / kTile;
     if (rows * tiles > 0x7fffffff)
       return qb::fail(QB_ERR_INVALID, "token_logprobs_bwd: too many rows");
