@@ -80,7 +80,8 @@ _SIGNATURES = {
     "qb_linear_ce_grad": [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
     "qb_pack_segment_size": [],
     "qb_adapter_pack": [_p, _i32, _i64, _p],
-    "qb_token_logprobs": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p],
+    "qb_token_logprobs_workspace": [_i64, _i64, _i32],
+    "qb_token_logprobs": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p, _p],
     "qb_token_logprobs_bwd": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p,
                               _p, _p],
     "qb_preference_config_size": [],
@@ -101,6 +102,7 @@ _RESTYPE = {"qb_last_error": ctypes.c_char_p, "qb_nf4_double_quant_workspace": c
             "qb_linear_ce_vocab_tiles": ctypes.c_int64,
             "qb_gemm_bf16_acc_f32_workspace": ctypes.c_int64,
             "qb_pack_segment_size": ctypes.c_int64, "qb_mask_job_size": ctypes.c_int64,
+            "qb_token_logprobs_workspace": ctypes.c_int64,
             "qb_preference_config_size": ctypes.c_int64,
             "qb_preference_workspace": ctypes.c_int64,
             "qb_policy_config_size": ctypes.c_int64, "qb_policy_workspace": ctypes.c_int64,

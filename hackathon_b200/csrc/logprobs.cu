@@ -14,17 +14,19 @@
 // A banned token (a logit of -inf) has e = 0 and no e d term: d is held at -300 T, where e is 0 and
 // every product with d finite. Rows need no other care: one of equal lowest values is the uniform distribution, one of -inf
 // alone, with +inf or with NaN is NaN, as the formula is.
-#include <cooperative_groups.h>
-
+#include <algorithm>
 #include <cstring>
 
 #include "qb_common.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace {
 
-constexpr int kThreads = 512;
+// 128 threads and 8 KB a batch: many small CTAs on an SM are each at another point of their row, so
+// loads and exponentials overlap (4096 x 152064 bf16: 189 us, 205 us with 512 threads and as many
+// bytes an SM in flight; with the entropy 196 and 227).
+constexpr int kFwdThreads = 128;
+constexpr int kFwdVectors = 4;         // 16-byte vectors per thread and batch
+constexpr int64_t kFwdCtas = 8 * 148;  // what the SMs hold at once
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float y) {
@@ -76,14 +78,16 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return r;
 }
 
-// 16 bytes of logits as pairs of fp32 values, and their maximum (a NaN stays one).
+// 16 bytes of logits: pair k of them less m, in fp32, and their maximum (a NaN stays one). The
+// 16-bit types are widened inside the subtraction (one instruction for both).
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
   uint4 u;
-  __device__ __forceinline__ Pair at(int k) const {
-    return k == 0 ? pair(__uint_as_float(u.x), __uint_as_float(u.y))
-                  : pair(__uint_as_float(u.z), __uint_as_float(u.w));
+  __device__ __forceinline__ Pair less(int k, float m) const {
+    const Pair z = k == 0 ? pair(__uint_as_float(u.x), __uint_as_float(u.y))
+                          : pair(__uint_as_float(u.z), __uint_as_float(u.w));
+    return add2(z, pair(-m, -m));
   }
   __device__ __forceinline__ float top() const {
     return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
@@ -103,6 +107,8 @@ template <typename T, typename H2> struct Vec16Bit {
   __device__ __forceinline__ uint32_t word(int k) const {
     return k == 0 ? u.x : k == 1 ? u.y : k == 2 ? u.z : u.w;
   }
+  __device__ __forceinline__ uint16_t low(int k) const { return word(k) & 0xffffu; }
+  __device__ __forceinline__ uint16_t high(int k) const { return word(k) >> 16; }
   __device__ __forceinline__ float top() const {
     const H2 m = __hmax2_nan(__hmax2_nan(word_as<H2>(u.x), word_as<H2>(u.y)),
                              __hmax2_nan(word_as<H2>(u.z), word_as<H2>(u.w)));
@@ -110,16 +116,20 @@ template <typename T, typename H2> struct Vec16Bit {
   }
 };
 template <> struct Vec<__nv_bfloat16> : Vec16Bit<__nv_bfloat16, __nv_bfloat162> {
-  __device__ __forceinline__ Pair at(int k) const {
-    const uint32_t w = word(k);
-    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  __device__ __forceinline__ Pair less(int k, float m) const {
+    float lo, hi;
+    asm("add.rn.f32.bf16 %0, %1, %2;" : "=f"(lo) : "h"(low(k)), "f"(-m));
+    asm("add.rn.f32.bf16 %0, %1, %2;" : "=f"(hi) : "h"(high(k)), "f"(-m));
+    return pair(lo, hi);
   }
   static __device__ __forceinline__ uint32_t none() { return 0xff80ff80u; }
 };
 template <> struct Vec<__half> : Vec16Bit<__half, __half2> {
-  __device__ __forceinline__ Pair at(int k) const {
-    const float2 f = __half22float2(word_as<__half2>(word(k)));
-    return pair(f.x, f.y);
+  __device__ __forceinline__ Pair less(int k, float m) const {
+    float lo, hi;
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(lo) : "h"(low(k)), "f"(-m));
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(hi) : "h"(high(k)), "f"(-m));
+    return pair(lo, hi);
   }
   static __device__ __forceinline__ uint32_t none() { return 0xfc00fc00u; }
 };
@@ -169,14 +179,14 @@ __device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scal
   for (int u = 1; u < U; ++u) m = max_nan(m, x[u].top());
   if (m == -INFINITY) return;    // all banned: nothing to add, and no maximum to subtract
   if (m > st.m) rescale(st, m, c);
-  const Pair minus = pair(-st.m, -st.m), cc = pair(c.c, c.c);
+  const Pair cc = pair(c.c, c.c);
   Pair s = pair(st.s, 0.f), t = pair(st.t, 0.f);
+  float lo, hi;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
 #pragma unroll
     for (int k = 0; k < Vec<T>::N / 2; ++k) {
-      Pair d = add2(x[u].at(k), minus);
-      float lo, hi;
+      const Pair d = x[u].less(k, st.m);
       halves(mul2(d, cc), lo, hi);
       const Pair e = pair(ex2(lo), ex2(hi));
       s = add2(s, e);
@@ -186,7 +196,6 @@ __device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scal
       }
     }
   }
-  float lo, hi;
   halves(s, lo, hi);
   st.s = lo + hi;
   halves(t, lo, hi);
@@ -203,89 +212,105 @@ __device__ __forceinline__ void add_one(Stat& st, float z, Scale c) {
   if (ENT) st.t += e * d;
 }
 
-// One CTA per row, or a cluster of CTAs when there are few rows: each takes every CS-th vector
-// block of the row, the cluster's first CTA merges.
+// One CTA per (row, span of the vocabulary): batches of kFwdVectors vectors a thread, the next one
+// requested before the present one is added up. The CTA's record goes to `partials`, or, where
+// one span is the whole row, straight to the outputs.
+struct Outputs {
+  const int64_t* target;
+  float* logp;
+  float* entropy;      // NULL: not asked for
+  float2* stats;
+};
+
+template <typename T>
+__device__ __forceinline__ void finish(const Outputs& out, int64_t row, const T* z, int vocab,
+                                       float inv_t, Stat st) {
+  const int64_t label = out.target[row];
+  const float log_s = logf(st.s);
+  float lp = 0.f;
+  if (label >= 0 && label < vocab) lp = (qb::to_f(z[label]) - st.m) * inv_t - log_s;
+  out.logp[row] = lp;
+  if (out.entropy) out.entropy[row] = log_s - inv_t * (st.t / st.s);
+  out.stats[row] = make_float2(st.m, st.s);
+}
+
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kThreads)
-token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab,
-                      const int64_t* __restrict__ target, float inv_t,
-                      float* __restrict__ logp, float* __restrict__ entropy,
-                      float2* __restrict__ stats) {
+__global__ void __launch_bounds__(kFwdThreads)
+token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab, int spans, int batches,
+                      float inv_t, Outputs out, float4* __restrict__ partials) {
   constexpr int VE = Vec<T>::N;
-  constexpr int U = 4;
-  __shared__ Stat warp_stat[32];
-  __shared__ Stat cta_stat;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cs = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int64_t row = blockIdx.x / cs;
+  constexpr int U = kFwdVectors;
+  __shared__ Stat warp_stat[kFwdThreads / 32];
+  const int64_t row = blockIdx.x / spans;
+  const int span = blockIdx.x % spans;
   const T* z = logits + rows.offset(row);
   const Scale c(inv_t);
-  const int tid = rank * kThreads + threadIdx.x, nthreads = cs * kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
-  // scalars before the first 16-byte boundary and after the last, vectors between
+  // scalars before the first 16-byte boundary and after the last (the first span takes them),
+  // vectors between; a thread past the end adds banned tokens
   const int head = min(vocab, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15)
                                                / sizeof(T)));
   const int nvec = (vocab - head) / VE;
   const T* body = z + head;
-
-  auto cluster_merge = [&](Stat st) {
-    st = warp_merge(st, c);
-    if (lane == 0) warp_stat[warp] = st;
-    __syncthreads();
-    if (warp == 0) {
-      st = lane < kThreads / 32 ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-      st = warp_merge(st, c);
-      if (lane == 0) cta_stat = st;
-    }
-    if (cs == 1) {
-      __syncthreads();
-      return cta_stat;
-    }
-    cluster.sync();
-    Stat all = *cluster.map_shared_rank(&cta_stat, 0);
-    for (int k = 1; k < cs; ++k) all = merge(all, *cluster.map_shared_rank(&cta_stat, k), c);
-    cluster.sync();            // nobody leaves, or writes again, while another still reads
-    return all;
-  };
-
-  Stat st{-INFINITY, 0.f, 0.f};
   const uint4 none = {Vec<T>::none(), Vec<T>::none(), Vec<T>::none(), Vec<T>::none()};
+  const int first = span * batches * (kFwdThreads * U) + threadIdx.x;
+  const int end = min(nvec, first + batches * (kFwdThreads * U));
   auto load = [&](Vec<T>(&x)[U], int v) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      x[u].u = v + u * nthreads < nvec
-                   ? __ldg(reinterpret_cast<const uint4*>(body + int64_t(v + u * nthreads) * VE))
+      x[u].u = v + u * kFwdThreads < end
+                   ? __ldg(reinterpret_cast<const uint4*>(body + int64_t(v + u * kFwdThreads) * VE))
                    : none;
   };
+  Stat st{-INFINITY, 0.f, 0.f};
   Vec<T> x[U], next[U];
-  load(x, tid);
-  for (int v = tid; v < nvec; v += U * nthreads) {
-    load(next, v + U * nthreads);      // in flight while this batch is added up
+  load(x, first);
+  for (int v = first; v < end; v += U * kFwdThreads) {
+    load(next, v + U * kFwdThreads);
     add_vectors<T, ENT, U>(st, x, c);
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = next[u];
   }
-  for (int j = tid; j < vocab - nvec * VE; j += nthreads)
+  if (span == 0 && static_cast<int>(threadIdx.x) < vocab - nvec * VE) {
+    const int j = threadIdx.x;
     add_one<ENT>(st, qb::to_f(z[j < head ? j : nvec * VE + j]), c);
-  st = cluster_merge(st);
-  if (rank == 0 && threadIdx.x == 0) {
-    const int64_t label = target[row];
-    const float log_s = logf(st.s);
-    float lp = 0.f;
-    if (label >= 0 && label < vocab) lp = (qb::to_f(z[label]) - st.m) * inv_t - log_s;
-    logp[row] = lp;
-    if (ENT) entropy[row] = log_s - inv_t * (st.t / st.s);
-    stats[row] = make_float2(st.m, st.s);
   }
+  st = warp_merge(st, c);
+  if (lane == 0) warp_stat[warp] = st;
+  __syncthreads();
+  if (warp != 0) return;
+  st = lane < kFwdThreads / 32 ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+  st = warp_merge(st, c);
+  if (lane != 0) return;
+  if (spans == 1) finish(out, row, z, vocab, inv_t, st);
+  else partials[blockIdx.x] = make_float4(st.m, st.s, st.t, 0.f);
+}
+
+// A warp per row: the row's records, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+token_logprobs_merge_kernel(const T* __restrict__ logits, Rows rows, int64_t n, int vocab,
+                            int spans, float inv_t, Outputs out,
+                            const float4* __restrict__ partials) {
+  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= n) return;
+  const int lane = threadIdx.x & 31;
+  const Scale c(inv_t);
+  Stat st{-INFINITY, 0.f, 0.f};
+  for (int k = lane; k < spans; k += 32) {
+    const float4 p = partials[row * spans + k];
+    st = merge(st, Stat{p.x, p.y, p.z}, c);
+  }
+  st = warp_merge(st, c);
+  if (lane == 0) finish(out, row, logits + rows.offset(row), vocab, inv_t, st);
 }
 
 // ---------------------------------------------------------------------------------------------
 // backward: elementwise given the row's (m, s, H); one CTA per (row, tile of columns)
 
-constexpr int kBwdThreads = 256;
-constexpr int kBwdVectors = 8;         // per thread and tile: 32 KB of logits a CTA
+constexpr int kThreads = 256;
+constexpr int kVectors = 8;            // per thread, all requested at once: 32 KB of logits a CTA
 
 __device__ __forceinline__ uint32_t packed(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -308,17 +333,17 @@ struct RowGrad {
     const float d = max_nan(z - m, c.low);
     return ex2(d * c.c) * fmaf(b, d, a);
   }
-  __device__ __forceinline__ void two(Pair z, float& lo, float& hi) const {
+  __device__ __forceinline__ void two(Pair less, float& lo, float& hi) const {
     float x, y;
-    halves(add2(z, pair(-m, -m)), x, y);
+    halves(less, x, y);
     const Pair d = pair(max_nan(x, c.low), max_nan(y, c.low));
     halves(mul2(d, pair(c.c, c.c)), x, y);
     halves(mul2(pair(ex2(x), ex2(y)), fma2(pair(b, b), d, pair(a, a))), lo, hi);
   }
   __device__ __forceinline__ uint4 vec(const Vec<float>& x) const {
     float f[4];
-    two(x.at(0), f[0], f[1]);
-    two(x.at(1), f[2], f[3]);
+    two(x.less(0, m), f[0], f[1]);
+    two(x.less(1, m), f[2], f[3]);
     return {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
             __float_as_uint(f[3])};
   }
@@ -328,7 +353,7 @@ struct RowGrad {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       float lo, hi;
-      two(x.at(k), lo, hi);
+      two(x.less(k, m), lo, hi);
       w[k] = packed(lo, hi, T());
     }
     return {w[0], w[1], w[2], w[3]};
@@ -336,14 +361,14 @@ struct RowGrad {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads)
+__global__ void __launch_bounds__(kThreads)
 token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, int tiles,
                           const int64_t* __restrict__ target, float inv_t,
                           const float2* __restrict__ stats, const float* __restrict__ entropy,
                           const float* __restrict__ g_logp, const float* __restrict__ g_ent,
                           T* __restrict__ dlogits) {
   constexpr int VE = Vec<T>::N;
-  constexpr int U = kBwdVectors;
+  constexpr int U = kVectors;
   const int64_t row = blockIdx.x / tiles;
   const int tile = blockIdx.x % tiles;
   const T* z = logits + rows.offset(row);
@@ -358,14 +383,14 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
   const int head = min(vocab, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dz) & 15)) & 15)
                                                / sizeof(T)));
   const int nvec = (vocab - head) / VE;
-  const int v0 = tile * (kBwdThreads * U) + threadIdx.x;
+  const int v0 = tile * (kThreads * U) + threadIdx.x;
   if (zero) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v0 + u * kBwdThreads < nvec)
-        *reinterpret_cast<uint4*>(dz + head + int64_t(v0 + u * kBwdThreads) * VE) = {0, 0, 0, 0};
+      if (v0 + u * kThreads < nvec)
+        *reinterpret_cast<uint4*>(dz + head + int64_t(v0 + u * kThreads) * VE) = {0, 0, 0, 0};
     if (tile == 0)
-      for (int j = threadIdx.x; j < vocab - nvec * VE; j += kBwdThreads)
+      for (int j = threadIdx.x; j < vocab - nvec * VE; j += kThreads)
         dz[j < head ? j : nvec * VE + j] = qb::from_f<T>(0.f);
     return;
   }
@@ -373,7 +398,7 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
   Vec<T> x[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int v = v0 + u * kBwdThreads;
+    const int v = v0 + u * kThreads;
     if (v < nvec) {
       const T* p = z + head + int64_t(v) * VE;
       if (vec_in) {
@@ -396,7 +421,7 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
   const int hot_vec = hot_col >= head && hot_col < head + nvec * VE ? (hot_col - head) / VE : -1;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int v = v0 + u * kBwdThreads;
+    const int v = v0 + u * kThreads;
     if (v < nvec) {
       const uint4 out = grad.vec(x[u]);
       *reinterpret_cast<uint4*>(dz + head + int64_t(v) * VE) = out;
@@ -404,11 +429,26 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, Rows rows, int vocab, in
     }
   }
   if (tile == 0) {
-    for (int j = threadIdx.x; j < vocab - nvec * VE; j += kBwdThreads) {
+    for (int j = threadIdx.x; j < vocab - nvec * VE; j += kThreads) {
       const int col = j < head ? j : nvec * VE + j;
       dz[col] = qb::from_f<T>(grad.one(qb::to_f(z[col])) + (col == hot_col ? hot : 0.f));
     }
   }
+}
+
+// Spans of a row and batches of a span: whole rows when they fill the SMs' slots, else rows are
+// cut until they do, down to a batch a CTA. Cutting further evens out the last wave but pays a
+// reduction and a record for each span: 999 rows of 50001 fp32 take 33 us whole and 36 to 38 cut
+// into 4 to 9 spans; 148 rows of 151936 bf16 take 14.7 us in 8 spans, 17.7 us in 2.
+struct Spans {
+  int64_t spans, batches;
+};
+Spans spans_of(int64_t rows, int64_t vocab, int e) {
+  const int64_t batch = int64_t(kFwdThreads) * kFwdVectors * (16 / e);
+  const int64_t all = (vocab + batch - 1) / batch;
+  const int64_t want = std::min(all, std::max<int64_t>(1, kFwdCtas / rows));
+  const int64_t batches = (all + want - 1) / want;
+  return {(all + batches - 1) / batches, batches};
 }
 
 int check(const char* what, const void* logits, int64_t rows, int64_t inner, int64_t vocab,
@@ -426,37 +466,44 @@ int check(const char* what, const void* logits, int64_t rows, int64_t inner, int
 
 }  // namespace
 
+extern "C" int64_t qb_token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype) {
+  const int e = qb::elem_size(dtype);
+  if (rows <= 0 || vocab <= 0 || e == 0) return 0;
+  const int64_t spans = spans_of(rows, vocab, e).spans;
+  return spans > 1 ? rows * spans * static_cast<int64_t>(sizeof(float4)) : 0;
+}
+
 extern "C" int qb_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t inner,
                                  int64_t stride_outer, int64_t stride_inner, int64_t vocab,
                                  const int64_t* target, float temperature, float* logp,
-                                 float* entropy, float* stats, cudaStream_t stream) {
+                                 float* entropy, float* stats, void* workspace,
+                                 cudaStream_t stream) {
   if (int rc = check("token_logprobs", logits, rows, inner, vocab, target, temperature, stats))
     return rc;
   if (rows == 0) return QB_OK;
-  if (!logp) return qb::fail(QB_ERR_INVALID, "token_logprobs: null pointer");
-  int cs = 1;
-  while (cs < 8 && rows * cs < 296 && vocab / cs > 8 * kThreads) cs *= 2;
-  if (rows * cs > 0x7fffffff) return qb::fail(QB_ERR_INVALID, "token_logprobs: too many rows");
   const Rows r{inner, stride_outer, stride_inner};
   const float inv_t = 1.f / temperature;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * cs));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(cs), 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  const Outputs out{target, logp, entropy, reinterpret_cast<float2*>(stats)};
+  auto* partials = static_cast<float4*>(workspace);
   QB_DISPATCH_FLOAT(dtype, T, {
-    auto* lp = static_cast<const T*>(logits);
-    auto* st = reinterpret_cast<float2*>(stats);
+    const Spans sp = spans_of(rows, vocab, sizeof(T));
+    if (!logp || (sp.spans > 1 && !workspace))
+      return qb::fail(QB_ERR_INVALID, "token_logprobs: null pointer");
+    if (rows > 0x7fffffff / sp.spans)
+      return qb::fail(QB_ERR_INVALID, "token_logprobs: too many rows");
+    const auto* z = static_cast<const T*>(logits);
+    const unsigned grid = static_cast<unsigned>(rows * sp.spans);
+    const int spans = static_cast<int>(sp.spans), batches = static_cast<int>(sp.batches);
     if (entropy)
-      cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, lp, r, (int)vocab, target, inv_t,
-                         logp, entropy, st);
+      token_logprobs_kernel<T, true><<<grid, kFwdThreads, 0, stream>>>(
+          z, r, (int)vocab, spans, batches, inv_t, out, partials);
     else
-      cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, lp, r, (int)vocab, target, inv_t,
-                         logp, entropy, st);
+      token_logprobs_kernel<T, false><<<grid, kFwdThreads, 0, stream>>>(
+          z, r, (int)vocab, spans, batches, inv_t, out, partials);
+    if (int rc = qb::check_launch("token_logprobs")) return rc;
+    if (spans > 1)
+      token_logprobs_merge_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(
+          z, r, rows, (int)vocab, spans, inv_t, out, partials);
   });
   return qb::check_launch("token_logprobs");
 }
@@ -474,11 +521,11 @@ extern "C" int qb_token_logprobs_bwd(const void* logits, int dtype, int64_t rows
     return qb::fail(QB_ERR_INVALID, "token_logprobs_bwd: null pointer");
   const Rows r{inner, stride_outer, stride_inner};
   QB_DISPATCH_FLOAT(dtype, T, {
-    constexpr int kTile = kBwdThreads * kBwdVectors * (16 / sizeof(T));
+    constexpr int64_t kTile = int64_t(kThreads) * kVectors * Vec<T>::N;
     const int64_t tiles = (vocab + kTile - 1) / kTile;
-    if (rows * tiles > 0x7fffffff)
+    if (rows > 0x7fffffff / tiles)
       return qb::fail(QB_ERR_INVALID, "token_logprobs_bwd: too many rows");
-    token_logprobs_bwd_kernel<T><<<static_cast<unsigned>(rows * tiles), kBwdThreads, 0, stream>>>(
+    token_logprobs_bwd_kernel<T><<<static_cast<unsigned>(rows * tiles), kThreads, 0, stream>>>(
         static_cast<const T*>(logits), r, (int)vocab, (int)tiles, target, 1.f / temperature,
         reinterpret_cast<const float2*>(stats), entropy, g_logp, g_entropy,
         static_cast<T*>(dlogits));

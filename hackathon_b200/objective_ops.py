@@ -92,29 +92,39 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, temperature, with_entropy):
         with _below_autograd():
-            logp, entropy, stats = token_logprobs(logits, target, temperature, with_entropy)
-        ctx.save_for_backward(logits, target, stats, entropy if with_entropy else None)
+            logp, entropy, state = token_logprobs(logits, target, temperature, with_entropy)
+        ctx.save_for_backward(logits, target, state, entropy if with_entropy else None)
         ctx.temperature, ctx.with_entropy = temperature, with_entropy
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*((stats,) if with_entropy else (entropy, stats)))
-        return logp, entropy, stats
+        ctx.mark_non_differentiable(*((state,) if with_entropy else (entropy, state)))
+        return logp, entropy, state
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g_logp, g_entropy, _g_stats):
-        logits, target, stats, entropy = ctx.saved_tensors
+    def backward(ctx, g_logp, g_entropy, _g_state):
+        logits, target, state, entropy = ctx.saved_tensors
         if not ctx.with_entropy:
             g_entropy = None
         if g_logp is None and g_entropy is None:
             return None, None, None, None
-        return token_logprobs_bwd(logits, target, stats, entropy, g_logp, g_entropy,
+        return token_logprobs_bwd(logits, target, state, entropy, g_logp, g_entropy,
                                   ctx.temperature), None, None, None
 
 
+def logprobs_state(rows, vocab, dtype):
+    """Floats of the op's third output: each row's (max, sum), then (16-byte aligned) the
+    kernels' workspace; and the workspace's offset."""
+    at = (2 * rows + 3) // 4 * 4
+    return at + _lib.load().qb_token_logprobs_workspace(rows, vocab, _lib.tag(dtype)) // 4, at
+
+
 def _token_logprobs_fake(logits, target, temperature, with_entropy):
+    rows, tile = target.numel(), 32768 // logits.element_size()
+    tiles = (logits.shape[-1] + tile - 1) // tile
     return (target.new_empty(target.shape, dtype=F32),
             target.new_empty(target.shape if with_entropy else (0,), dtype=F32),
-            target.new_empty((target.numel(), 2), dtype=F32))
+            target.new_empty(((2 * rows + 3) // 4 * 4 + (4 * rows * tiles if tiles > 1 else 0),),
+                             dtype=F32))
 
 
 @_register("token_logprobs(Tensor logits, Tensor target, float temperature, bool with_entropy) "
@@ -124,20 +134,22 @@ def token_logprobs(logits, target, temperature, with_entropy):
     vocab, dev = logits.shape[-1], logits.device
     logp = torch.empty(target.shape, dtype=F32, device=dev)
     entropy = torch.empty(target.shape if with_entropy else (0,), dtype=F32, device=dev)
-    stats = torch.empty((rows, 2), dtype=F32, device=dev)
+    size, at = logprobs_state(rows, vocab, z.dtype)
+    state = torch.empty(size, dtype=F32, device=dev)
     if rows:
         tgt = target.contiguous()
         _lib.call_on(dev, "qb_token_logprobs", z.data_ptr(), _lib.tag(z.dtype), rows, inner, so,
                      si, vocab, tgt.data_ptr(), temperature, logp.data_ptr(),
-                     entropy.data_ptr() if with_entropy else None, stats.data_ptr(),
+                     entropy.data_ptr() if with_entropy else None, state.data_ptr(),
+                     state.data_ptr() + 4 * at, kernels=2 if size > at else 1,
                      work=(rows * (vocab * z.element_size() + 20), 0))
-    return logp, entropy, stats
+    return logp, entropy, state
 
 
-@_register("token_logprobs_bwd(Tensor logits, Tensor target, Tensor stats, Tensor? entropy, "
+@_register("token_logprobs_bwd(Tensor logits, Tensor target, Tensor state, Tensor? entropy, "
            "Tensor? g_logp, Tensor? g_entropy, float temperature) -> Tensor",
            lambda logits, *_: logits.new_empty(logits.shape))
-def token_logprobs_bwd(logits, target, stats, entropy, g_logp, g_entropy, temperature):
+def token_logprobs_bwd(logits, target, state, entropy, g_logp, g_entropy, temperature):
     z, rows, inner, so, si = row_layout(logits)
     vocab, dev = logits.shape[-1], logits.device
     out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
@@ -146,7 +158,7 @@ def token_logprobs_bwd(logits, target, stats, entropy, g_logp, g_entropy, temper
         gl = g_logp.contiguous() if g_logp is not None else None
         ge = g_entropy.contiguous() if g_entropy is not None else None
         _lib.call_on(dev, "qb_token_logprobs_bwd", z.data_ptr(), _lib.tag(z.dtype), rows, inner,
-                     so, si, vocab, tgt.data_ptr(), temperature, stats.data_ptr(),
+                     so, si, vocab, tgt.data_ptr(), temperature, state.data_ptr(),
                      _lib.ptr(entropy), _lib.ptr(gl), _lib.ptr(ge), out.data_ptr(),
                      work=(rows * (2 * vocab * z.element_size() + 28), 0))
     return out

@@ -451,16 +451,20 @@ int qb_selftest_bounded_wait(int64_t limit_ns, cudaStream_t stream);
  * Post-training objectives and gradient clipping (no counterpart in the reference)
  */
 
+/* Bytes of workspace qb_token_logprobs needs (0: none). */
+int64_t qb_token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype);
+
 /* Per row of logits: logp = (z[label] - m) / T - ln sum exp((z - m) / T) with m the row's maximum
  * (0 for labels outside [0, vocab)), and, when `entropy` is given, the entropy of the row's
  * distribution. Row r of `rows` starts at (r / inner) * stride_outer + (r % inner) *
  * stride_inner elements, so a [batch, positions, vocab] view needs no copy; the last dimension
- * is contiguous. stats [rows, 2] (8-byte aligned) receives (m, sum) for the backward. Logits of
- * -inf have probability 0; a row of nothing else is NaN. T in 1e-6 .. 1e6. */
+ * is contiguous. stats [rows, 2] (8-byte aligned) receives (m, sum) for the backward; workspace is 16-byte
+ * aligned device memory. Logits of -inf have probability 0; a row of nothing else is NaN. T in
+ * 1e-6 .. 1e6. */
 int qb_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t inner,
                       int64_t stride_outer, int64_t stride_inner, int64_t vocab,
                       const int64_t* target, float temperature, float* logp, float* entropy,
-                      float* stats, cudaStream_t stream);
+                      float* stats, void* workspace, cudaStream_t stream);
 
 /* dlogits [rows, vocab] (contiguous, the logits' dtype) of the sum of g_logp * logp + g_entropy *
  * entropy: (g (onehot - p) - g_entropy p (ln p + entropy)) / T. g_logp or g_entropy may be NULL

@@ -68,6 +68,11 @@ def test_state_layout_matches_the_library(n, cols):
     assert lib.qb_preference_config_size() == ctypes.sizeof(oo.PreferenceConfig)
     assert lib.qb_policy_config_size() == ctypes.sizeof(oo.PolicyConfig)
     meta = torch.empty(n, cols, device="meta")
+    for dtype in (torch.float32, torch.bfloat16):
+        size, at = oo.logprobs_state(n, cols, dtype)
+        assert at >= 2 * n and at % 4 == 0
+        target = torch.empty(n, device="meta", dtype=torch.int64)
+        assert oo._token_logprobs_fake(meta.to(dtype), target, 1.0, True)[2].shape == (size,)
     size, at = oo.preference_state(n, cols)
     assert at >= 2 * n and at % 4 == 0
     assert oo._preference_fake(meta)[1].shape == (size,)
@@ -112,7 +117,7 @@ def test_c_entries_refuse_before_any_launch():
 
     def lp(rows=4, inner=1, vocab=10, t=1.0, dtype=0, logits=fake, out=fake):
         return ("qb_token_logprobs", logits, dtype, rows, inner, vocab, 0, vocab, fake, t, out,
-                None, fake, None)
+                None, fake, fake, None)
 
     cases = [(lp(vocab=0), "bad shape"), (lp(rows=-1), "bad shape"), (lp(inner=0), "bad shape"),
              (lp(inner=3), "bad shape"), (lp(vocab=1 << 30), "bad shape"),
@@ -180,7 +185,7 @@ def test_c_entries_refuse_before_any_launch():
             _lib.call(*args)
     # nothing to do is no error
     assert _lib.load().qb_token_logprobs(None, 0, 0, 1, 10, 0, 10, None, 1.0, None, None, None,
-                                         None) == 0
+                                         None, None) == 0
     assert _lib.load().qb_preference_workspace(0, 5) == 0
     assert _lib.load().qb_policy_workspace(4, 0) == 0
 
