@@ -5,7 +5,7 @@
 //
 // The tensors' addresses and sizes travel in the kernel's parameters (up to 1600 tensors a
 // launch), so nothing is copied to the device and a captured launch keeps its own table. The
-// tensors are cut into chunks of kChunk elements; a fixed grid walks the chunks, each CTA adds
+// tensors are cut into chunks of 32 KB; a fixed grid walks the chunks, each CTA adds
 // its own in 64 bits and writes one partial sum, and whoever needs the norm adds the partials in
 // order: the same bits on every run. 64-bit sums of 64-bit squares: no gradient's square
 // overflows or is lost, and HBM still bounds it (two 64-bit operations for each 2 or 4 bytes).
@@ -20,9 +20,11 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kChunk = 8192;         // elements: 32 KB of fp32, 16 KB of the 16-bit types
+constexpr int kChunkBytes = 32 * 1024;   // eight 16-byte vectors a thread, all in flight at once
+__host__ __device__ constexpr int64_t chunk_of(int e) { return kChunkBytes / e; }   // elements
 constexpr int kMaxTensors = 1600;        // per launch: the table stays under 32 KB of parameters
-constexpr int kMaxGrid = 1184;           // 8 CTAs of 256 threads on each of 148 SMs
+constexpr int kMaxGrid = 592;            // of the norm: 4 CTAs of 256 threads on each of 148 SMs
+constexpr int kClipGrid = 1184;          // of the scaling: 8 on each, of which 3 at once
 
 template <int K>
 struct Table {
@@ -47,18 +49,25 @@ __device__ __forceinline__ Part part_of(const Table<K>& t, int chunk) {
   }
   const int64_t size = t.size[lo] >> 2;
   const int dtype = static_cast<int>(t.size[lo] & 3);
-  const int64_t start = int64_t(chunk - t.first[lo]) * kChunk;
+  const int e = dtype == QB_F32 ? 4 : 2;
+  const int64_t start = int64_t(chunk - t.first[lo]) * chunk_of(e);
   const int64_t left = size - start;
-  return {static_cast<char*>(t.ptr[lo]) + start * (dtype == QB_F32 ? 4 : 2),
-          static_cast<int>(left < kChunk ? left : kChunk), dtype};
+  return {static_cast<char*>(t.ptr[lo]) + start * e,
+          static_cast<int>(left < chunk_of(e) ? left : chunk_of(e)), dtype};
 }
 
-// acc over the elements of one norm: sum x^2, sum |x| or max |x| (a NaN stays).
+// What a thread gathers of one norm: sum x^2 or sum |x| in 64 bits, or max |x| (a NaN stays).
+template <int P> struct Sum {
+  using type = double;
+};
+template <> struct Sum<0> {
+  using type = float;
+};
 template <int P>
-__device__ __forceinline__ void take(double& acc, float x) {
-  if (P == 2) acc = fma(static_cast<double>(x), static_cast<double>(x), acc);
-  else if (P == 1) acc += static_cast<double>(fabsf(x));
-  else acc = x != x || acc != acc ? NAN : fmax(acc, static_cast<double>(fabsf(x)));
+__device__ __forceinline__ void take(typename Sum<P>::type& acc, float x) {
+  if constexpr (P == 2) acc = fma(static_cast<double>(x), static_cast<double>(x), acc);
+  else if constexpr (P == 1) acc += static_cast<double>(fabsf(x));
+  else asm("max.NaN.f32 %0, %1, %2;" : "=f"(acc) : "f"(acc), "f"(fabsf(x)));
 }
 
 template <int P>
@@ -88,9 +97,9 @@ __device__ __forceinline__ int head_of(const T* p, int len) {
 }
 
 template <typename T, int P>
-__device__ __forceinline__ void norm_part(double& acc, const T* p, int len) {
+__device__ __forceinline__ void norm_part(typename Sum<P>::type& acc, const T* p, int len) {
   constexpr int VE = 16 / sizeof(T);
-  constexpr int U = static_cast<int>(kChunk) / VE / kThreads;
+  constexpr int U = kChunkBytes / 16 / kThreads;
   const int head = head_of(p, len), nvec = (len - head) / VE;
   qb::Vec16<T> x[U];
 #pragma unroll
@@ -109,16 +118,17 @@ __device__ __forceinline__ void norm_part(double& acc, const T* p, int len) {
 template <int K, int P>
 __global__ void __launch_bounds__(kThreads)
 grad_norm_kernel(const __grid_constant__ Table<K> table, double* __restrict__ partials) {
+  qb::release_next();
   __shared__ double scratch[32];
-  double acc = 0.0;
+  typename Sum<P>::type acc = 0;
   for (int c = blockIdx.x; c < table.chunks; c += gridDim.x) {
     const Part part = part_of(table, c);
     if (part.dtype == QB_F32) norm_part<float, P>(acc, static_cast<const float*>(part.p), part.len);
     else if (part.dtype == QB_F16) norm_part<__half, P>(acc, static_cast<const __half*>(part.p), part.len);
     else norm_part<__nv_bfloat16, P>(acc, static_cast<const __nv_bfloat16*>(part.p), part.len);
   }
-  acc = block_join<P>(acc, scratch);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  const double all = block_join<P>(acc, scratch);
+  if (threadIdx.x == 0) partials[blockIdx.x] = all;
 }
 
 // The norm from the partials, the same in every thread of every CTA.
@@ -133,6 +143,7 @@ __device__ double total_norm(const double* __restrict__ partials, int n, int p, 
 __global__ void __launch_bounds__(kThreads)
 grad_norm_total_kernel(const double* __restrict__ partials, int n, int p,
                        float* __restrict__ norm) {
+  qb::await_previous();
   __shared__ double scratch[32];
   const double v = total_norm(partials, n, p, scratch);
   if (threadIdx.x == 0) *norm = static_cast<float>(v);
@@ -141,13 +152,13 @@ grad_norm_total_kernel(const double* __restrict__ partials, int n, int p,
 template <typename T>
 __device__ __forceinline__ void scale_part(T* p, int len, float coef) {
   constexpr int VE = 16 / sizeof(T);
-  constexpr int U = static_cast<int>(kChunk) / VE / kThreads;
+  constexpr int U = kChunkBytes / 16 / kThreads;
   const int head = head_of(p, len), nvec = (len - head) / VE;
   qb::Vec16<T> x[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int v = threadIdx.x + u * kThreads;
-    if (v < nvec) x[u].u = *reinterpret_cast<const uint4*>(p + head + v * VE);
+    if (v < nvec) x[u].u = __ldcs(reinterpret_cast<const uint4*>(p + head + v * VE));
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -155,7 +166,7 @@ __device__ __forceinline__ void scale_part(T* p, int len, float coef) {
     if (v < nvec) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) x[u].v[e] = qb::from_f<T>(qb::to_f(x[u].v[e]) * coef);
-      *reinterpret_cast<uint4*>(p + head + v * VE) = x[u].u;
+      __stcs(reinterpret_cast<uint4*>(p + head + v * VE), x[u].u);
     }
   }
   for (int j = threadIdx.x; j < len - nvec * VE; j += kThreads) {
@@ -168,6 +179,7 @@ template <int K>
 __global__ void __launch_bounds__(kThreads)
 grad_clip_kernel(const __grid_constant__ Table<K> table, const double* __restrict__ partials,
                  int n, int p, double max_norm, float* __restrict__ norm) {
+  qb::await_previous();
   __shared__ double scratch[32];
   const double v = total_norm(partials, n, p, scratch);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(v);
@@ -222,17 +234,17 @@ int check_overlap(const char* what, const Args& a) {
   return QB_OK;
 }
 
-// Calls launch(table, grid) for tensors [*at, ...) as long as they fit one table, and moves *at on.
+// Calls launch(table, grid of at most `most` CTAs) for tensors [*at, ...) as long as they fit one table, and moves *at on.
 template <int K, typename F>
-int launch_table(const Args& a, int64_t* at, F&& launch) {
+int launch_table(const Args& a, int64_t* at, int most, F&& launch) {
   Table<K> t;
   t.n = 0;
   int64_t chunks = 0;
   for (; *at < a.n && t.n < K; ++*at) {
     const int64_t size = a.sizes[*at];
     if (size == 0) continue;
-    const int64_t c = (size + kChunk - 1) / kChunk;
-    if (chunks + c > 0x7fff0000) break;           // 1.7e13 elements: the next launch's
+    const int64_t chunk = chunk_of(qb::elem_size(a.dtypes[*at])), c = (size + chunk - 1) / chunk;
+    if (chunks + c > 0x7fff0000) break;           // more than 1.7e13 elements: the next launch's
     t.ptr[t.n] = reinterpret_cast<void*>(a.ptrs[*at]);
     t.size[t.n] = size << 2 | a.dtypes[*at];
     t.first[t.n] = static_cast<int32_t>(chunks);
@@ -241,15 +253,15 @@ int launch_table(const Args& a, int64_t* at, F&& launch) {
   }
   t.chunks = static_cast<int32_t>(chunks);
   if (t.n == 0) return QB_OK;
-  return launch(t, static_cast<int>(std::min<int64_t>(chunks, kMaxGrid)));
+  return launch(t, static_cast<int>(std::min<int64_t>(chunks, most)));
 }
 
 template <typename F>
-int launch_all(const Args& a, F&& launch) {
+int launch_all(const Args& a, int most, F&& launch) {
   for (int64_t at = 0; at < a.n;) {
     const int64_t left = a.n - at;
-    const int rc = left <= 96 ? launch_table<96>(a, &at, launch)
-                              : launch_table<kMaxTensors>(a, &at, launch);
+    const int rc = left <= 96 ? launch_table<96>(a, &at, most, launch)
+                              : launch_table<kMaxTensors>(a, &at, most, launch);
     if (rc) return rc;
   }
   return QB_OK;
@@ -258,7 +270,7 @@ int launch_all(const Args& a, F&& launch) {
 int norm_partials(const Args& a, int p, double* partials, int64_t capacity, int64_t* used,
                   cudaStream_t stream) {
   *used = 0;
-  return launch_all(a, [&](const auto& t, int grid) {
+  return launch_all(a, kMaxGrid, [&](const auto& t, int grid) {
     if (*used + grid > capacity)
       return qb::fail(QB_ERR_INVALID, "grad_norm: workspace of %lld sums is too small",
                       (long long)capacity);
@@ -294,7 +306,8 @@ extern "C" int qb_grad_norm(const uint64_t* ptrs, const int64_t* sizes, const ui
   if (int rc = check_norm("grad_norm", a, order, workspace, norm)) return rc;
   int64_t used = 0;
   if (int rc = norm_partials(a, order, workspace, workspace_doubles, &used, stream)) return rc;
-  grad_norm_total_kernel<<<1, kThreads, 0, stream>>>(workspace, static_cast<int>(used), order, norm);
+  qb::launch_after(grad_norm_total_kernel, 1, kThreads, stream, workspace, static_cast<int>(used),
+                   order, norm);
   return qb::check_launch("grad_norm");
 }
 
@@ -317,11 +330,16 @@ extern "C" int qb_grad_clip(const uint64_t* ptrs, const int64_t* sizes, const ui
                                      norm, stream);
   const double limit = *max_norm;
   float* out = norm;                     // the first launch writes it
-  return launch_all(a, [&](const auto& t, int grid) {
+  return launch_all(a, kClipGrid, [&](const auto& t, int grid) {
     using Tab = std::decay_t<decltype(t)>;
     constexpr int K = sizeof(Tab::size) / sizeof(int64_t);
-    grad_clip_kernel<K><<<grid, kThreads, 0, stream>>>(t, workspace, static_cast<int>(used), order,
-                                                       limit, out);
+    // directly behind the last norm launch; a further table's launch waits for the one before
+    if (out)
+      qb::launch_after(grad_clip_kernel<K>, grid, kThreads, stream, t, workspace,
+                       static_cast<int>(used), order, limit, out);
+    else
+      grad_clip_kernel<K><<<grid, kThreads, 0, stream>>>(t, workspace, static_cast<int>(used),
+                                                         order, limit, out);
     out = nullptr;
     return qb::check_launch("grad_clip");
   });

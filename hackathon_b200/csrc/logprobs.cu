@@ -241,6 +241,7 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab, int sp
   constexpr int VE = Vec<T>::N;
   constexpr int U = kFwdVectors;
   __shared__ Stat warp_stat[kFwdThreads / 32];
+  qb::release_next();
   const int64_t row = blockIdx.x / spans;
   const int span = blockIdx.x % spans;
   const T* z = logits + rows.offset(row);
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(256)
 token_logprobs_merge_kernel(const T* __restrict__ logits, Rows rows, int64_t n, int vocab,
                             int spans, float inv_t, Outputs out,
                             const float4* __restrict__ partials) {
+  qb::await_previous();
   const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= n) return;
   const int lane = threadIdx.x & 31;
@@ -502,8 +504,8 @@ extern "C" int qb_token_logprobs(const void* logits, int dtype, int64_t rows, in
           z, r, (int)vocab, spans, batches, inv_t, out, partials);
     if (int rc = qb::check_launch("token_logprobs")) return rc;
     if (spans > 1)
-      token_logprobs_merge_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(
-          z, r, rows, (int)vocab, spans, inv_t, out, partials);
+      qb::launch_after(token_logprobs_merge_kernel<T>, static_cast<unsigned>((rows + 7) / 8), 256,
+                       stream, z, r, rows, (int)vocab, spans, inv_t, out, partials);
   });
   return qb::check_launch("token_logprobs");
 }

@@ -11,21 +11,33 @@ constexpr int kObjThreads = 256;
 constexpr int kObjPerThread = 8;
 constexpr int kObjChunk = kObjThreads * kObjPerThread;   // columns per CTA
 
-__device__ __forceinline__ double warp_sum64(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Sum over the block in a fixed order; every thread gets it. `scratch` holds 32 doubles.
-__device__ __forceinline__ double block_sum64(double v, double* scratch) {
+// N sums over the block at once, in a fixed order; every thread gets them. `scratch` holds 32 * N
+// doubles.
+template <int N>
+__device__ __forceinline__ void block_sums64(double (&v)[N], double* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nwarps = (blockDim.x + 31) >> 5;
-  v = warp_sum64(v);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   __syncthreads();  // scratch may still be read by a previous call
-  if (lane == 0) scratch[warp] = v;
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) scratch[k * 32 + warp] = v[k];
   __syncthreads();
-  return warp_sum64(lane < nwarps ? scratch[lane] : 0.0);
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = lane < nwarps ? scratch[k * 32 + lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+}
+
+__device__ __forceinline__ double block_sum64(double v, double* scratch) {
+  double a[1] = {v};
+  block_sums64(a, scratch);
+  return a[0];
 }
 
 // Lanes that share a row's records in the adding CTA: a power of two, so that a row of few

@@ -7,8 +7,8 @@
 //   token:     sum mask L / denominator            (default: the number of unmasked tokens)
 //   sequence:  sum_i (sum_t mask L / max(n_i, 1)) / denominator    (default: the rows)
 //
-// The gradient jumps where r crosses a border, so the side is decided on l in 64 bits against the
-// borders' logarithms, not on a rounded r. k3 cancels for small d: below |d| = 1/2 it is summed
+// The gradient jumps where r crosses a border, so the side is decided on l against the borders'
+// logarithms, not on a rounded r, and in 64 bits wherever l is near one. k3 cancels for small d: below |d| = 1/2 it is summed
 // as its Taylor series. The forward writes each token's dL/dlogp (fp32, unnormalised) when a
 // gradient will be asked for; the backward multiplies it by g and the row's weight. Sums are
 // 64-bit, in a fixed order. Masked places are skipped, whatever they hold.
@@ -25,10 +25,15 @@ using qb::kObjThreads;
 // What the kernels take of qb_policy_config.
 struct Params {
   double log_low, log_high, log_delta;   // the borders of r as logarithms
+  float log_low32, log_high32, log_delta32;
   float low, high, delta, kl_coef;
   double denominator;
   bool sequence;
 };
+
+// l = logp - old in fp32 is off by 2^-24 |l| and a border by as much: beyond 1e-5 (borders up to
+// e^+-80, further than fp32's exponential reaches) both say the same as their 64-bit forms.
+constexpr float kNear = 1e-5f;
 
 struct Record {
   double loss, kl;
@@ -63,7 +68,8 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
                    int64_t adv_col, const uint8_t* __restrict__ mask, int64_t cols, int chunks,
                    Params par, Record* __restrict__ records,
                    float* __restrict__ unit) {
-  __shared__ double scratch[32];
+  qb::release_next();
+  __shared__ double scratch[96];
   const int64_t row = blockIdx.x / chunks, base = row * cols;
   const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
   float lp[kObjPerThread], lo[kObjPerThread], lr[kObjPerThread], av[kObjPerThread];
@@ -84,19 +90,24 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
   for (int k = 0; k < kObjPerThread; ++k) {
     float g = 0.f;
     if (on[k]) {
-      const double l = static_cast<double>(lp[k]) - static_cast<double>(lo[k]);
-      const float r = expf(static_cast<float>(l)), a = av[k];
+      const float l = lp[k] - lo[k], a = av[k];       // the 64-bit difference, rounded once
+      bool below = l < par.log_low32, above = l > par.log_high32, past = l > par.log_delta32;
+      if (fabsf(l - par.log_low32) < kNear || fabsf(l - par.log_high32) < kNear ||
+          fabsf(l - par.log_delta32) < kNear) {
+        const double exact = static_cast<double>(lp[k]) - static_cast<double>(lo[k]);
+        below = exact < par.log_low;
+        above = exact > par.log_high;
+        past = exact > par.log_delta;
+      }
+      const float r = expf(l);
       const float first = fminf(r, par.delta), held = fminf(fmaxf(r, par.low), par.high);
       float term = -fminf(first * a, held * a);
       if (r != r || a != a) term = r * a;
-      const bool below = l < par.log_low, above = l > par.log_high;
-      bool live = !(below || above) || (below && a > 0.f) || (above && a < 0.f);
-      live = live && l <= par.log_delta;
+      const bool live = !past && (!(below || above) || (below && a > 0.f) || (above && a < 0.f));
       g = live ? -a * r : 0.f;
       if (ref) {
         float k3, em1;
-        kl_terms(static_cast<float>(static_cast<double>(lr[k]) - static_cast<double>(lp[k])), k3,
-                 em1);
+        kl_terms(lr[k] - lp[k], k3, em1);
         term = fmaf(par.kl_coef, k3, term);
         g = fmaf(-par.kl_coef, em1, g);
         kl += k3;
@@ -109,14 +120,12 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
     const int64_t col = c0 + k * kObjThreads;
     if (unit && col < cols) unit[base + col] = g;
   }
-  loss = qb::block_sum64(loss, scratch);
-  if (ref) kl = qb::block_sum64(kl, scratch);
   // the three counts of a chunk in one exact double: each is at most kObjChunk = 2^11 < 2^16
-  const double packed = qb::block_sum64(
-      count + low * 65536.0 + high * 4294967296.0, scratch);
+  double sums[3] = {loss, count + low * 65536.0 + high * 4294967296.0, kl};
+  qb::block_sums64(sums, scratch);
   if (threadIdx.x == 0) {
-    const int64_t p = static_cast<int64_t>(packed);
-    records[blockIdx.x] = Record{loss, kl, static_cast<int32_t>(p & 0xffff),
+    const int64_t p = static_cast<int64_t>(sums[1]);
+    records[blockIdx.x] = Record{sums[0], sums[2], static_cast<int32_t>(p & 0xffff),
                                  static_cast<int32_t>((p >> 16) & 0xffff),
                                  static_cast<int32_t>(p >> 32), 0};
   }
@@ -129,7 +138,8 @@ __global__ void __launch_bounds__(1024)
 policy_total_kernel(const Record* __restrict__ records, int chunks, int lanes, int64_t rows,
                     Params par, const double* __restrict__ denom_dev, float* __restrict__ loss,
                     float* __restrict__ stats, float* __restrict__ weight) {
-  __shared__ double scratch[32];
+  qb::await_previous();
+  __shared__ double scratch[160];
   double total = 0.0, kl = 0.0, count = 0.0, low = 0.0, high = 0.0;
   const bool given = denom_dev || par.denominator > 0;
   const double asked = denom_dev ? *denom_dev : par.denominator;
@@ -161,12 +171,10 @@ policy_total_kernel(const Record* __restrict__ records, int chunks, int lanes, i
       weight[r] = static_cast<float>(1.0 / (each * per));
     }
   }
-  total = qb::block_sum64(total, scratch);
-  kl = qb::block_sum64(kl, scratch);
-  count = qb::block_sum64(count, scratch);
-  low = qb::block_sum64(low, scratch);
-  high = qb::block_sum64(high, scratch);
+  double all[5] = {total, kl, count, low, high};
+  qb::block_sums64(all, scratch);
   if (threadIdx.x == 0) {
+    total = all[0], kl = all[1], count = all[2], low = all[3], high = all[4];
     const double tokens = fmax(count, 1.0);
     const double denom = par.sequence ? per : given ? asked : tokens;
     *loss = static_cast<float>(total / denom);
@@ -240,6 +248,9 @@ extern "C" int qb_policy_fwd(const void* logp, const void* old_logp, const void*
   par.log_low = log1p(-cfg->clip_low);        // -inf for a lower border of 0
   par.log_high = log1p(cfg->clip_high);
   par.log_delta = cfg->delta > 0 ? log(cfg->delta) : INFINITY;
+  par.log_low32 = static_cast<float>(par.log_low);
+  par.log_high32 = static_cast<float>(par.log_high);
+  par.log_delta32 = static_cast<float>(par.log_delta);
   par.low = static_cast<float>(1.0 - cfg->clip_low);
   par.high = static_cast<float>(1.0 + cfg->clip_high);
   par.delta = cfg->delta > 0 ? static_cast<float>(cfg->delta) : INFINITY;
@@ -253,8 +264,8 @@ extern "C" int qb_policy_fwd(const void* logp, const void* old_logp, const void*
   });
   if (int rc = qb::check_launch("policy")) return rc;
   const int lanes = qb::lanes_per_row(chunks);
-  policy_total_kernel<<<1, qb::adding_threads(rows, lanes), 0, stream>>>(
-      records, chunks, lanes, rows, par, denominator, loss, stats, weight);
+  qb::launch_after(policy_total_kernel, 1, qb::adding_threads(rows, lanes), stream, records,
+                   chunks, lanes, rows, par, denominator, loss, stats, weight);
   return qb::check_launch("policy");
 }
 

@@ -28,7 +28,8 @@ __global__ void __launch_bounds__(kObjThreads)
 preference_rows_kernel(const T* __restrict__ logp, const T* __restrict__ ref,
                        const uint8_t* __restrict__ mask, int64_t cols, int chunks,
                        Record* __restrict__ records) {
-  __shared__ double scratch[32];
+  qb::release_next();
+  __shared__ double scratch[64];
   const int64_t row = blockIdx.x / chunks, base = row * cols;
   const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
   float a[kObjPerThread], b[kObjPerThread];
@@ -49,9 +50,9 @@ preference_rows_kernel(const T* __restrict__ logp, const T* __restrict__ ref,
       ++count;
     }
   }
-  sum = qb::block_sum64(sum, scratch);
-  const double n = qb::block_sum64(count, scratch);
-  if (threadIdx.x == 0) records[blockIdx.x] = Record{sum, static_cast<int64_t>(n)};
+  double both[2] = {sum, static_cast<double>(count)};
+  qb::block_sums64(both, scratch);
+  if (threadIdx.x == 0) records[blockIdx.x] = Record{both[0], static_cast<int64_t>(both[1])};
 }
 
 // NaN in, NaN out: fabs keeps it, and log1p(exp()) carries it.
@@ -67,6 +68,7 @@ preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lane
                         const float* __restrict__ ref_row, qb_preference_config cfg,
                         const double* __restrict__ denom_dev, float* __restrict__ loss,
                         float* __restrict__ rewards, float* __restrict__ coef) {
+  qb::await_previous();
   __shared__ double scratch[32];
   const double denom = denom_dev ? *denom_dev
                                  : cfg.denominator > 0 ? cfg.denominator : double(pairs);
@@ -175,8 +177,8 @@ extern "C" int qb_preference_fwd(const void* logp, const void* ref, int dtype,
   });
   if (int rc = qb::check_launch("preference")) return rc;
   const int lanes = qb::lanes_per_row(chunks);
-  preference_pairs_kernel<<<1, qb::adding_threads(pairs, lanes), 0, stream>>>(
-      records, chunks, lanes, pairs, ref_row, *cfg, denominator, loss, rewards, coef);
+  qb::launch_after(preference_pairs_kernel, 1, qb::adding_threads(pairs, lanes), stream, records,
+                   chunks, lanes, pairs, ref_row, *cfg, denominator, loss, rewards, coef);
   return qb::check_launch("preference");
 }
 

@@ -138,6 +138,34 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
   return warp_sum(t);
 }
 
+// ---------------------------------------------------------------------------------------------
+// A second launch that follows up on the first (programmatic dependent launch): it is set up while
+// the first still runs, once every CTA of that one has called release_next(), and its own CTAs
+// call await_previous() before they touch memory. Only for a kernel directly behind the one it
+// follows up on.
+
+__device__ __forceinline__ void release_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void await_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+inline void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream,
+                         A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);   // check_launch sees its error
+}
+
 }  // namespace qb
 
 // Dispatch over the three floating dtypes of the C-ABI.
