@@ -193,8 +193,13 @@ def call(name, *args, work=(0, 0), kernels=1):
     else:
         status = getattr(lib, name)(*args)
     if status != 0:
-        msg = lib.qb_last_error().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (status {status}): {msg}")
+        raise_last(lib, name, status)
+
+
+def raise_last(lib, name, status):
+    """Raises the message of this thread's last failed call."""
+    msg = lib.qb_last_error().decode(errors="replace")
+    raise RuntimeError(f"{name} failed (status {status}): {msg}")
 
 
 def call_on(device, name, *args, work=(0, 0), kernels=1):
@@ -204,6 +209,12 @@ def call_on(device, name, *args, work=(0, 0), kernels=1):
     at = here if device.index is None else device.index
     raw = torch._C._cuda_getCurrentRawStream(at)     # stream(device) without the Stream object
     if at == here:
+        if _timer is None:
+            lib = _lib or load()
+            status = getattr(lib, name)(*args, raw)
+            if status != 0:
+                raise_last(lib, name, status)
+            return
         return call(name, *args, raw, work=work, kernels=kernels)
     with torch.cuda.device(at):
         return call(name, *args, raw, work=work, kernels=kernels)

@@ -29,28 +29,31 @@ from .ops import NS
 
 F32 = torch.float32
 _library = torch.library.Library(NS, "FRAGMENT")
+_ops = getattr(torch.ops, NS)
 _below_autograd = torch._C._AutoDispatchBelowAutograd
 
 
-def _register(schema, fake, function=None, grad_arg=0):
+def _register(schema, fake, function=None):
     """Registers the decorated function as the CUDA kernel of the op `schema` declares, with its
-    fake implementation; `function`: the autograd.Function that calls it when the argument
-    numbered grad_arg asks for a gradient. Returns the op."""
+    fake implementation; `function`: the autograd.Function that calls it when the first argument
+    asks for a gradient. Returns what calls the op."""
     name = schema[:schema.index("(")]
 
     def register(kernel):
         _library.define(schema)
         _library.impl(name, kernel, "CUDA")
         torch.library.register_fake(f"{NS}::{name}", fake, lib=_library)
-        op = getattr(getattr(torch.ops, NS), name).default
-        if function is not None:
-            def autograd(*args):
-                if torch.is_grad_enabled() and args[grad_arg].requires_grad:
-                    return function.apply(*args)
-                with _below_autograd():
-                    return op(*args)
-            _library.impl(name, autograd, "Autograd")
-        return op
+        op = getattr(_ops, name).default
+        if function is None:
+            return op
+
+        def autograd(*args):
+            if torch.is_grad_enabled() and args[0].requires_grad:
+                return function.apply(*args)
+            with _below_autograd():
+                return op(*args)
+        _library.impl(name, autograd, "Autograd")
+        return autograd     # what the op does first, without the way through the dispatcher
     return register
 
 
@@ -92,7 +95,8 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, temperature, with_entropy):
         with _below_autograd():
-            logp, entropy, state = token_logprobs(logits, target, temperature, with_entropy)
+            logp, entropy, state = _ops.token_logprobs.default(logits, target, temperature,
+                                                               with_entropy)
         ctx.save_for_backward(logits, target, state, entropy if with_entropy else None)
         ctx.temperature, ctx.with_entropy = temperature, with_entropy
         ctx.set_materialize_grads(False)
@@ -111,20 +115,29 @@ class _TokenLogprobs(torch.autograd.Function):
                                   ctx.temperature), None, None, None
 
 
-def logprobs_state(rows, vocab, dtype):
-    """Floats of the op's third output: each row's (max, sum), then (16-byte aligned) the
-    kernels' workspace; and the workspace's offset."""
-    at = (2 * rows + 3) // 4 * 4
-    return at + _lib.load().qb_token_logprobs_workspace(rows, vocab, _lib.tag(dtype)) // 4, at
+# The second (or third) output of an op is one fp32 buffer: what its backward or the caller reads,
+# then, 16-byte aligned, the kernels' workspace. The sizes below are the library's
+# qb_*_workspace, written here too because a fake implementation needs them of symbolic sizes.
+
+
+def _up4(n):
+    return (n + 3) // 4 * 4
+
+
+def logprobs_state(rows, vocab, itemsize):
+    """Floats of the third output ((max, sum) of each row, workspace), the workspace's offset."""
+    at = _up4(2 * rows)
+    batch = 8192 // itemsize                       # elements a CTA reads at a time
+    batches = (vocab + batch - 1) // batch
+    spans = min(batches, max(1, 1184 // max(rows, 1)))
+    return at + (4 * rows * spans if spans > 1 else 0), at
 
 
 def _token_logprobs_fake(logits, target, temperature, with_entropy):
-    rows, tile = target.numel(), 32768 // logits.element_size()
-    tiles = (logits.shape[-1] + tile - 1) // tile
+    size, _ = logprobs_state(target.numel(), logits.shape[-1], logits.element_size())
     return (target.new_empty(target.shape, dtype=F32),
             target.new_empty(target.shape if with_entropy else (0,), dtype=F32),
-            target.new_empty(((2 * rows + 3) // 4 * 4 + (4 * rows * tiles if tiles > 1 else 0),),
-                             dtype=F32))
+            target.new_empty((size,), dtype=F32))
 
 
 @_register("token_logprobs(Tensor logits, Tensor target, float temperature, bool with_entropy) "
@@ -134,7 +147,7 @@ def token_logprobs(logits, target, temperature, with_entropy):
     vocab, dev = logits.shape[-1], logits.device
     logp = torch.empty(target.shape, dtype=F32, device=dev)
     entropy = torch.empty(target.shape if with_entropy else (0,), dtype=F32, device=dev)
-    size, at = logprobs_state(rows, vocab, z.dtype)
+    size, at = logprobs_state(rows, vocab, z.element_size())
     state = torch.empty(size, dtype=F32, device=dev)
     if rows:
         tgt = target.contiguous()
@@ -172,7 +185,7 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, mask, *args):
         with _below_autograd():
-            loss, state = preference(logp, mask, *args)
+            loss, state = _ops.preference.default(logp, mask, *args)
         ctx.save_for_backward(mask, state)
         ctx.shape, ctx.dtype, ctx.args = logp.shape, logp.dtype, len(args)
         ctx.set_materialize_grads(False)
@@ -190,17 +203,15 @@ class _Preference(torch.autograd.Function):
 
 
 def preference_state(n, cols):
-    """Floats of the op's second output: rewards [n], coefficients [n], then (16-byte aligned)
-    the kernels' workspace; and the workspace's offset."""
-    at = (2 * n + 3) // 4 * 4
-    return at + _lib.load().qb_preference_workspace(n // 2, cols) // 4, at
+    """Floats of the second output (rewards [n], coefficients [n], workspace), the workspace's
+    offset."""
+    at = _up4(2 * n)
+    return at + 4 * n * ((cols + 2047) // 2048), at
 
 
 def _preference_fake(logp, *_):
-    # the workspace's size is the library's to say; what is read of the state are its first 2n
-    n, cols = logp.shape
-    return logp.new_empty((), dtype=F32), logp.new_empty(
-        ((2 * n + 3) // 4 * 4 + n * ((cols + 2047) // 2048) * 4,), dtype=F32)
+    return logp.new_empty((), dtype=F32), logp.new_empty((preference_state(*logp.shape)[0],),
+                                                         dtype=F32)
 
 
 @_register("preference(Tensor logp, Tensor? mask, Tensor? ref, Tensor? ref_row, "
@@ -245,7 +256,7 @@ class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, *args):
         with _below_autograd():
-            loss, state, unit = policy(logp, *args)
+            loss, state, unit = _ops.policy.default(logp, *args)
         ctx.save_for_backward(state, unit)
         ctx.dtype, ctx.args, ctx.sequence, ctx.with_grad = logp.dtype, len(args), *args[-2:]
         ctx.set_materialize_grads(False)
@@ -266,18 +277,17 @@ class _Policy(torch.autograd.Function):
 
 
 def policy_state(n, cols, sequence):
-    """Floats of the op's second output: statistics [4], weights (one, or [n]), then (16-byte
-    aligned) the kernels' workspace; and the workspace's offset."""
-    at = (4 + (n if sequence else 1) + 3) // 4 * 4
-    return at + _lib.load().qb_policy_workspace(n, cols) // 4, at
+    """Floats of the second output (statistics [4], weights [n] or one, workspace), the workspace's
+    offset."""
+    at = _up4(4 + (n if sequence else 1))
+    return at + 8 * n * ((cols + 2047) // 2048), at
 
 
 def _policy_fake(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_high, delta,
                  kl_coef, divide_by, sequence, with_grad):
     n, cols = logp.shape
-    at = (4 + (n if sequence else 1) + 3) // 4 * 4
     return (logp.new_empty((), dtype=F32),
-            logp.new_empty((at + n * ((cols + 2047) // 2048) * 8,), dtype=F32),
+            logp.new_empty((policy_state(n, cols, sequence)[0],), dtype=F32),
             logp.new_empty((n if with_grad else 0, cols), dtype=F32))
 
 

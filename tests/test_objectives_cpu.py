@@ -62,23 +62,30 @@ def test_gradients_have_the_inputs_shapes_on_meta_tensors():
         torch.autograd.grad(g.sum(), x)
 
 
-@pytest.mark.parametrize("n,cols", [(2, 1), (6, 2048), (6, 2049), (10, 70001)])
+@pytest.mark.parametrize("n,cols", [(2, 1), (6, 2048), (6, 2049), (10, 70001), (2, 151936),
+                                    (300, 50001), (592, 8193), (1184, 40000), (5000, 152064)])
 def test_state_layout_matches_the_library(n, cols):
+    """The buffers the ops allocate hold what the library says its workspace needs, at an aligned
+    offset, and the fake implementations give their sizes."""
     lib = _lib.load()
     assert lib.qb_preference_config_size() == ctypes.sizeof(oo.PreferenceConfig)
     assert lib.qb_policy_config_size() == ctypes.sizeof(oo.PolicyConfig)
     meta = torch.empty(n, cols, device="meta")
-    for dtype in (torch.float32, torch.bfloat16):
-        size, at = oo.logprobs_state(n, cols, dtype)
+    target = torch.empty(n, device="meta", dtype=I64)
+    for dtype, tag in ((F32, 0), (torch.float16, 1), (BF, 2)):
+        size, at = oo.logprobs_state(n, cols, dtype.itemsize)
         assert at >= 2 * n and at % 4 == 0
-        target = torch.empty(n, device="meta", dtype=torch.int64)
+        assert 4 * (size - at) >= lib.qb_token_logprobs_workspace(n, cols, tag)
+        assert (size > at) >= (lib.qb_token_logprobs_workspace(n, cols, tag) > 0)
         assert oo._token_logprobs_fake(meta.to(dtype), target, 1.0, True)[2].shape == (size,)
     size, at = oo.preference_state(n, cols)
     assert at >= 2 * n and at % 4 == 0
+    assert 4 * (size - at) == lib.qb_preference_workspace(n // 2, cols)
     assert oo._preference_fake(meta)[1].shape == (size,)
     for sequence in (False, True):
         size, at = oo.policy_state(n, cols, sequence)
         assert at >= 4 + (n if sequence else 1) and at % 4 == 0
+        assert 4 * (size - at) == lib.qb_policy_workspace(n, cols)
         got = oo._policy_fake(meta, *(None,) * 10, sequence, True)
         assert got[1].shape == (size,) and got[2].shape == (n, cols)
 
