@@ -11,9 +11,9 @@ constexpr int kObjThreads = 256;
 constexpr int kObjPerThread = 8;
 constexpr int kObjChunk = kObjThreads * kObjPerThread;   // columns per CTA
 
-// N sums over the block at once, in a fixed order; every thread gets them. `scratch` holds 32 * N
-// doubles.
-template <int N>
+// N sums over the block at once, in a fixed order; every thread gets them, or with FIRST only the
+// first warp's. `scratch` holds 32 * N doubles.
+template <bool FIRST = false, int N>
 __device__ __forceinline__ void block_sums64(double (&v)[N], double* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nwarps = (blockDim.x + 31) >> 5;
@@ -26,6 +26,7 @@ __device__ __forceinline__ void block_sums64(double (&v)[N], double* scratch) {
 #pragma unroll
     for (int k = 0; k < N; ++k) scratch[k * 32 + warp] = v[k];
   __syncthreads();
+  if (FIRST && warp != 0) return;
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = lane < nwarps ? scratch[k * 32 + lane] : 0.0;
 #pragma unroll

@@ -7,8 +7,9 @@
 //   token:     sum mask L / denominator            (default: the number of unmasked tokens)
 //   sequence:  sum_i (sum_t mask L / max(n_i, 1)) / denominator    (default: the rows)
 //
-// The gradient jumps where r crosses a border, so the side is decided on l against the borders'
-// logarithms, not on a rounded r, and in 64 bits wherever l is near one. k3 cancels for small d: below |d| = 1/2 it is summed
+// The gradient jumps where r crosses a border, so the side is that of the exact l against the
+// border's logarithm B, not of a rounded r. Rounding keeps the order: the fp32 difference says which
+// side it is wherever it is not B's own rounding, and there the 64-bit difference does. k3 cancels for small d: below |d| = 1/2 it is summed
 // as its Taylor series. The forward writes each token's dL/dlogp (fp32, unnormalised) when a
 // gradient will be asked for; the backward multiplies it by g and the row's weight. Sums are
 // 64-bit, in a fixed order. Masked places are skipped, whatever they hold.
@@ -30,10 +31,6 @@ struct Params {
   double denominator;
   bool sequence;
 };
-
-// l = logp - old in fp32 is off by 2^-24 |l| and a border by as much: beyond 1e-5 (borders up to
-// e^+-80, further than fp32's exponential reaches) both say the same as their 64-bit forms.
-constexpr float kNear = 1e-5f;
 
 struct Record {
   double loss, kl;
@@ -70,19 +67,28 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
                    float* __restrict__ unit) {
   qb::release_next();
   __shared__ double scratch[96];
-  const int64_t row = blockIdx.x / chunks, base = row * cols;
-  const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
+  const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+  const int64_t c0 = int64_t(blockIdx.x % static_cast<unsigned>(chunks)) * kObjChunk + threadIdx.x;
+  const int64_t at = row * cols + c0;
+  const int left = static_cast<int>(cols - c0 < kObjChunk ? cols - c0 : kObjChunk);
+  logp += at;
+  old = old ? old + at : logp;           // the policy itself: l = 0
+  if (ref) ref += at;
+  if (mask) mask += at;
+  if (unit) unit += at;
+  adv += row * adv_row + c0 * adv_col;
+  const float adv_one = adv_col == 0 ? *adv : 0.f;
   float lp[kObjPerThread], lo[kObjPerThread], lr[kObjPerThread], av[kObjPerThread];
   bool on[kObjPerThread];
 #pragma unroll
   for (int k = 0; k < kObjPerThread; ++k) {
-    const int64_t col = c0 + k * kObjThreads;
-    const bool in = col < cols;
-    on[k] = in && (!mask || mask[base + col]);
-    lp[k] = in ? qb::to_f(logp[base + col]) : 0.f;
-    lo[k] = in && old ? qb::to_f(old[base + col]) : lp[k];
-    lr[k] = in && ref ? qb::to_f(ref[base + col]) : 0.f;
-    av[k] = in ? adv[row * adv_row + col * adv_col] : 0.f;
+    const int j = k * kObjThreads;
+    const bool in = j < left;
+    on[k] = in && (!mask || mask[j]);
+    lp[k] = in ? qb::to_f(logp[j]) : 0.f;
+    lo[k] = in ? qb::to_f(old[j]) : 0.f;
+    lr[k] = in && ref ? qb::to_f(ref[j]) : 0.f;
+    av[k] = adv_col == 0 ? adv_one : in ? adv[j * adv_col] : 0.f;
   }
   double loss = 0.0, kl = 0.0;
   int count = 0, low = 0, high = 0;
@@ -92,8 +98,7 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
     if (on[k]) {
       const float l = lp[k] - lo[k], a = av[k];       // the 64-bit difference, rounded once
       bool below = l < par.log_low32, above = l > par.log_high32, past = l > par.log_delta32;
-      if (fabsf(l - par.log_low32) < kNear || fabsf(l - par.log_high32) < kNear ||
-          fabsf(l - par.log_delta32) < kNear) {
+      if (l == par.log_low32 || l == par.log_high32 || l == par.log_delta32) {
         const double exact = static_cast<double>(lp[k]) - static_cast<double>(lo[k]);
         below = exact < par.log_low;
         above = exact > par.log_high;
@@ -108,8 +113,10 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
       if (ref) {
         float k3, em1;
         kl_terms(lr[k] - lp[k], k3, em1);
-        term = fmaf(par.kl_coef, k3, term);
-        g = fmaf(-par.kl_coef, em1, g);
+        if (par.kl_coef != 0.f) {          // 0 of an overflowed k3 is nothing
+          term = fmaf(par.kl_coef, k3, term);
+          g = fmaf(-par.kl_coef, em1, g);
+        }
         kl += k3;
       }
       loss += term;
@@ -117,19 +124,29 @@ policy_rows_kernel(const T* __restrict__ logp, const T* __restrict__ old,
       low += below && a < 0.f;
       high += above && a > 0.f;
     }
-    const int64_t col = c0 + k * kObjThreads;
-    if (unit && col < cols) unit[base + col] = g;
+    if (unit && k * kObjThreads < left) unit[k * kObjThreads] = g;
   }
-  // the three counts of a chunk in one exact double: each is at most kObjChunk = 2^11 < 2^16
-  double sums[3] = {loss, count + low * 65536.0 + high * 4294967296.0, kl};
-  qb::block_sums64(sums, scratch);
+  // the three counts of a warp (at most 2^8 each) in one integer, then of the chunk in one exact
+  // double (at most 2^11 each)
+  const unsigned counts = __reduce_add_sync(0xffffffffu, count + (low << 10) + (high << 20));
+  const double packed = threadIdx.x % 32 == 0 ? (counts & 1023) + (counts >> 10 & 1023) * 65536.0
+                                                    + (counts >> 20) * 4294967296.0 : 0.0;
+  double sums[3] = {loss, kl, packed};
+  if (ref) {
+    qb::block_sums64<true>(sums, scratch);
+  } else {
+    double two[2] = {loss, packed};
+    qb::block_sums64<true>(two, scratch);
+    sums[0] = two[0], sums[2] = two[1];
+  }
   if (threadIdx.x == 0) {
-    const int64_t p = static_cast<int64_t>(sums[1]);
-    records[blockIdx.x] = Record{sums[0], sums[2], static_cast<int32_t>(p & 0xffff),
+    const int64_t p = static_cast<int64_t>(sums[2]);
+    records[blockIdx.x] = Record{sums[0], sums[1], static_cast<int32_t>(p & 0xffff),
                                  static_cast<int32_t>((p >> 16) & 0xffff),
                                  static_cast<int32_t>(p >> 32), 0};
   }
 }
+static_assert(kObjPerThread * 32 < 1024, "a warp's counts are packed in ten bits each");
 
 // One CTA: a group of lanes per row, the records added in a fixed order. stats: tokens, mean k3,
 // the shares of the tokens held by the lower and by the upper border. weight: one number (token),
@@ -172,17 +189,21 @@ policy_total_kernel(const Record* __restrict__ records, int chunks, int lanes, i
     }
   }
   double all[5] = {total, kl, count, low, high};
-  qb::block_sums64(all, scratch);
-  if (threadIdx.x == 0) {
-    total = all[0], kl = all[1], count = all[2], low = all[3], high = all[4];
-    const double tokens = fmax(count, 1.0);
-    const double denom = par.sequence ? per : given ? asked : tokens;
-    *loss = static_cast<float>(total / denom);
-    if (!par.sequence) weight[0] = static_cast<float>(1.0 / denom);
-    stats[0] = static_cast<float>(count);
-    stats[1] = static_cast<float>(kl / tokens);
-    stats[2] = static_cast<float>(low / tokens);
-    stats[3] = static_cast<float>(high / tokens);
+  qb::block_sums64<true>(all, scratch);
+  if (threadIdx.x >= 32) return;
+  // a lane each for the five quotients
+  const double tokens = fmax(all[2], 1.0);
+  const double denom = par.sequence ? per : given ? asked : tokens;
+  const int k = threadIdx.x;
+  const float q = static_cast<float>((k == 0 ? all[0] : k == 1 ? 1.0 : k == 2 ? all[1]
+                                      : k == 3 ? all[3] : all[4]) / (k < 2 ? denom : tokens));
+  if (k == 0) {
+    *loss = q;
+    stats[0] = static_cast<float>(all[2]);
+  } else if (k == 1) {
+    if (!par.sequence) weight[0] = q;
+  } else if (k < 5) {
+    stats[k - 1] = q;
   }
 }
 
@@ -191,21 +212,21 @@ __global__ void __launch_bounds__(kObjThreads)
 policy_bwd_kernel(const float* __restrict__ unit, const float* __restrict__ weight,
                   int64_t weight_row, const float* __restrict__ g, int64_t cols, int chunks,
                   T* __restrict__ grad) {
-  const int64_t row = blockIdx.x / chunks, base = row * cols;
-  const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
+  const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+  const int64_t c0 = int64_t(blockIdx.x % static_cast<unsigned>(chunks)) * kObjChunk + threadIdx.x;
+  const int left = static_cast<int>(cols - c0 < kObjChunk ? cols - c0 : kObjChunk);
+  unit += row * cols + c0;
+  grad += row * cols + c0;
   const float w = weight[row * weight_row] * *g;
   float v[kObjPerThread];
 #pragma unroll
-  for (int k = 0; k < kObjPerThread; ++k) {
-    const int64_t col = c0 + k * kObjThreads;
-    v[k] = col < cols ? unit[base + col] : 0.f;
-  }
+  for (int k = 0; k < kObjPerThread; ++k)
+    v[k] = k * kObjThreads < left ? unit[k * kObjThreads] : 0.f;
 #pragma unroll
-  for (int k = 0; k < kObjPerThread; ++k) {
-    const int64_t col = c0 + k * kObjThreads;
+  for (int k = 0; k < kObjPerThread; ++k)
     // a token without a gradient (masked, or held by the clip) has none whatever g is
-    if (col < cols) grad[base + col] = qb::from_f<T>(v[k] == 0.f ? 0.f : v[k] * w);
-  }
+    if (k * kObjThreads < left)
+      grad[k * kObjThreads] = qb::from_f<T>(v[k] == 0.f ? 0.f : v[k] * w);
 }
 
 int check(const char* what, int64_t rows, int64_t cols) {

@@ -30,16 +30,20 @@ preference_rows_kernel(const T* __restrict__ logp, const T* __restrict__ ref,
                        Record* __restrict__ records) {
   qb::release_next();
   __shared__ double scratch[64];
-  const int64_t row = blockIdx.x / chunks, base = row * cols;
-  const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
+  const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+  const int64_t c0 = int64_t(blockIdx.x % static_cast<unsigned>(chunks)) * kObjChunk + threadIdx.x;
+  const int left = static_cast<int>(cols - c0 < kObjChunk ? cols - c0 : kObjChunk);
+  logp += row * cols + c0;
+  if (ref) ref += row * cols + c0;
+  if (mask) mask += row * cols + c0;
   float a[kObjPerThread], b[kObjPerThread];
   bool on[kObjPerThread];
 #pragma unroll
   for (int k = 0; k < kObjPerThread; ++k) {
-    const int64_t col = c0 + k * kObjThreads;
-    on[k] = col < cols && (!mask || mask[base + col]);
-    a[k] = col < cols ? qb::to_f(logp[base + col]) : 0.f;
-    b[k] = ref && col < cols ? qb::to_f(ref[base + col]) : 0.f;
+    const int j = k * kObjThreads;
+    on[k] = j < left && (!mask || mask[j]);
+    a[k] = j < left ? qb::to_f(logp[j]) : 0.f;
+    b[k] = ref && j < left ? qb::to_f(ref[j]) : 0.f;
   }
   double sum = 0.0;
   int count = 0;
@@ -50,8 +54,9 @@ preference_rows_kernel(const T* __restrict__ logp, const T* __restrict__ ref,
       ++count;
     }
   }
-  double both[2] = {sum, static_cast<double>(count)};
-  qb::block_sums64(both, scratch);
+  const unsigned n = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(count));
+  double both[2] = {sum, threadIdx.x % 32 == 0 ? static_cast<double>(n) : 0.0};
+  qb::block_sums64<true>(both, scratch);
   if (threadIdx.x == 0) records[blockIdx.x] = Record{both[0], static_cast<int64_t>(both[1])};
 }
 
@@ -117,8 +122,9 @@ preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lane
     coef[p] = static_cast<float>(slope / (denom * n[0]));
     coef[p + pairs] = static_cast<float>(-slope / (denom * n[1]));
   }
-  total = qb::block_sum64(total, scratch);
-  if (threadIdx.x == 0) *loss = static_cast<float>(total / denom);
+  double all[1] = {total};
+  qb::block_sums64<true>(all, scratch);
+  if (threadIdx.x == 0) *loss = static_cast<float>(all[0] / denom);
 }
 
 template <typename T>
@@ -126,13 +132,16 @@ __global__ void __launch_bounds__(kObjThreads)
 preference_bwd_kernel(const uint8_t* __restrict__ mask, const float* __restrict__ coef,
                       const float* __restrict__ g, int64_t cols, int chunks,
                       T* __restrict__ grad) {
-  const int64_t row = blockIdx.x / chunks, base = row * cols;
-  const int64_t c0 = int64_t(blockIdx.x % chunks) * kObjChunk + threadIdx.x;
+  const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+  const int64_t c0 = int64_t(blockIdx.x % static_cast<unsigned>(chunks)) * kObjChunk + threadIdx.x;
+  const int left = static_cast<int>(cols - c0 < kObjChunk ? cols - c0 : kObjChunk);
+  grad += row * cols + c0;
+  if (mask) mask += row * cols + c0;
   const T v = qb::from_f<T>(coef[row] * *g), zero = qb::from_f<T>(0.f);
 #pragma unroll
   for (int k = 0; k < kObjPerThread; ++k) {
-    const int64_t col = c0 + k * kObjThreads;
-    if (col < cols) grad[base + col] = !mask || mask[base + col] ? v : zero;
+    const int j = k * kObjThreads;
+    if (j < left) grad[j] = !mask || mask[j] ? v : zero;
   }
 }
 

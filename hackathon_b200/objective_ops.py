@@ -53,7 +53,10 @@ def _register(schema, fake, function=None):
             with _below_autograd():
                 return op(*args)
         _library.impl(name, autograd, "Autograd")
-        return autograd     # what the op does first, without the way through the dispatcher
+
+        def call(*args):    # what the op does first, without the way through the dispatcher
+            return op(*args) if torch.compiler.is_compiling() else autograd(*args)
+        return call
     return register
 
 

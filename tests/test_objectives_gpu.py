@@ -133,7 +133,7 @@ def test_preference_extremes(cuda):
     x = torch.tensor([[-1e6], [0.0], [0.0], [-1e6]], device=cuda, requires_grad=True)
     loss, _ = preference_loss(x, beta=1.0)
     (g,) = torch.autograd.grad(loss, x)
-    assert abs(float(loss) - 5e5) <= 2 * U * 5e5
+    assert abs(float(loss.detach()) - 5e5) <= 2 * U * 5e5
     assert g.flatten().tolist() == [-0.5, 0.0, 0.5, 0.0]
     mask = torch.zeros(4, 1, dtype=torch.bool, device=cuda)
     loss, step = preference_loss(x, mask, beta=1.0, length_normalized=True)
@@ -358,8 +358,78 @@ def test_policy_against_differences(cuda):
     assert abs(got - want) <= 20 * U * float((g.double() * d).abs().sum()) + 1e-6
 
 
+def test_policy_far_references(cuda):
+    """A reference so far away that e^d overflows: an infinite KL term where it counts, none at a
+    coefficient of 0; a token impossible under the reference costs infinitely much."""
+    from hackathon_b200.policy import policy_loss
+    x = torch.tensor([[-200.0, -1.0]], device=cuda, requires_grad=True)
+    one = torch.ones(1, device=cuda)
+    far = torch.zeros(1, 2, device=cuda)
+    loss, step = policy_loss(x, x.detach(), one, None, far, kl_coef=0.0)
+    (g,) = torch.autograd.grad(loss, x)
+    assert float(loss.detach()) == -1.0 and g.tolist() == [[-0.5, -0.5]]
+    assert float(step.kl) == math.inf
+    assert float(policy_loss(x, x.detach(), one, None, far, kl_coef=0.1)[0]) == math.inf
+    never = torch.tensor([[-200.0, -math.inf]], device=cuda)
+    assert float(policy_loss(x, x.detach(), one, None, never, kl_coef=0.1)[0]) == math.inf
+
+
 # ---------------------------------------------------------------------------------------------
 # both
+
+
+def test_compiled_functions_trace_the_operators(cuda):
+    """torch.compile sees the operators whole (no graph break) and gives the eager bits."""
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+    logp, mask, randn = draw(cuda, 6, 70, torch.float32, 81)
+    old, adv = logp + 0.2 * randn(6, 70), randn(6)
+    z, t = randn(6, 300), torch.arange(6, device=cuda)
+
+    def objective(x, logits):
+        a, _ = preference_loss(x, mask, old)
+        b, _ = policy_loss(x, old, adv, mask, old, kl_coef=0.1)
+        lp, en = token_logprobs(logits, t, 0.9, True)
+        return a + b + lp.sum() - en.sum()
+
+    def step(fn):
+        x, logits = logp.clone().requires_grad_(), z.clone().requires_grad_()
+        out = fn(x, logits)
+        return (out.detach(), *torch.autograd.grad(out, (x, logits)))
+
+    torch._dynamo.reset()
+    want = step(objective)
+    got = step(torch.compile(objective, backend="aot_eager", fullgraph=True))
+    assert all(map(torch.equal, got, want))
+
+
+@pytest.mark.parametrize("kind", ["preference", "policy"])
+def test_more_than_32_bits_of_tokens(cuda, kind):
+    """2.2 billion tokens: the values past 2^31 count and get their gradients."""
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+    n, s = 2, (1 << 30) + (1 << 26) + 7
+    x = torch.zeros(n, s, dtype=torch.bfloat16, device=cuda)
+    mask = torch.zeros(n, s, dtype=torch.bool, device=cuda)
+    at = [(0, 0), (0, s - 1), (1, 0), (1, (1 << 30) + 5), (1, s - 1)]
+    for k, (i, j) in enumerate(at):
+        x[i, j] = -1.0 - k
+        mask[i, j] = True
+    x.requires_grad_()
+    if kind == "preference":
+        loss, step = preference_loss(x, mask, beta=1.0)
+        assert [float(step.chosen_rewards), float(step.rejected_rewards)] == [-3.0, -12.0]
+        slope = -1 / (1 + math.exp(9.0))
+        want = [slope, slope, -slope, -slope, -slope]
+    else:
+        loss, step = policy_loss(x, None, torch.tensor([1.0, -2.0], device=cuda), mask)
+        assert float(step.tokens) == 5.0 and abs(float(loss.detach()) - 4 / 5) <= 2 * U
+        want = [-0.2, -0.2, 0.4, 0.4, 0.4]
+    (g,) = torch.autograd.grad(loss, x)
+    got = [float(g[i, j]) for i, j in at]
+    assert all(abs(a - b) <= (2.0 ** -8 + 4 * U) * abs(b) for a, b in zip(got, want))
+    assert int(torch.count_nonzero(g)) == 5
 
 
 @pytest.mark.parametrize("kind", ["preference", "policy"])
