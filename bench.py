@@ -65,7 +65,8 @@ BOUND = {"qb_nf4_dequant": "hbm", "qb_rmsnorm_fwd": "hbm", "qb_rmsnorm_bwd": "hb
          # the forward's gate/up GEMM with the next masks drawn in its side warps: its flops are
          # the GEMM's (the Philox rounds it also runs are counted under no roofline)
          "qb_gemm_gateup_swiglu_masks": "tensor",
-         "qb_dropout_mask": "hbm", "qb_dropout_apply": "hbm",
+         "qb_dropout_mask": "hbm", "qb_dropout_apply": "hbm", "qb_token_logprobs": "hbm",
+         "qb_token_logprobs_bwd": "hbm", "qb_grad_norm": "hbm", "qb_grad_clip": "hbm",
          # integer-pipe work (Philox rounds), counted in mask elements drawn: no HBM or tensor
          # roofline applies; on a side stream its events span the GEMMs it shares the SMs with
          "qb_dropout_bits": "philox"}
@@ -336,9 +337,10 @@ KERNELS = ("gemm2", "gemm_dgrad", "nf4_fwd_fused", "nf4_fwd_dequant", "nf4_dgrad
            "dropout_mask", "dropout_apply", "swiglu_fwd", "rmsnorm_fwd", "rmsnorm_bwd",
            "rope_bwd", "linear_ce", "mask_acc", "gateup_swiglu", "gemm2_dgrad_pair",
            "gemm2_rope", "dropout_bits", "lora_xa", "lora_xa_xd", "lora_grads",
-           "gateup_swiglu_masks")
+           "gateup_swiglu_masks", "token_logprobs", "token_logprobs_bwd", "grad_norm", "grad_clip")
 GRAPHABLE = ("nf4_dequant", "dropout_mask", "dropout_apply", "swiglu_fwd", "rmsnorm_fwd",
-             "rmsnorm_bwd", "rope_bwd", "dropout_bits")
+             "rmsnorm_bwd", "rope_bwd", "dropout_bits", "token_logprobs", "token_logprobs_bwd",
+             "grad_norm", "grad_clip")
 
 
 def kernel_case(args):
@@ -465,6 +467,32 @@ def kernel_case(args):
         _, bits = dropout_mask(dx, 0.05, 7, 1 / 0.95)
         fn = lambda: gemm_mask_acc(v, a_l.t(), bits, 1 / 0.95, dx)  # noqa: E731
         nbytes = 2 * T * fi * 2 + bits.numel() * 4 + T * r * 2 + r * fi * 2
+    elif name in ("token_logprobs", "token_logprobs_bwd"):
+        # --tokens rows of bf16 logits over a vocabulary of --out-features: log-probability and
+        # entropy, or the gradient of both
+        from hackathon_b200 import objective_ops as oo
+        z = rnd(T, fo, s=2.5)
+        tgt = torch.randint(0, fo, (T,), device=dev, generator=g)
+        lp, ent, state = oo.token_logprobs(z, tgt, 1.0, True)
+        if name == "token_logprobs":
+            fn = lambda: oo.token_logprobs(z, tgt, 1.0, True)  # noqa: E731
+            nbytes = T * (fo * 2 + 24)
+        else:
+            fn = lambda: oo.token_logprobs_bwd(z, tgt, state, ent, lp, ent, 1.0)  # noqa: E731
+            nbytes = T * (2 * fo * 2 + 28)
+    elif name in ("grad_norm", "grad_clip"):
+        # fp32 gradients of --tokens tensors of --in-features x 64 elements; the clipping's limit
+        # is below its formula's 1e-6, so every launch scales
+        from hackathon_b200.grad_norm import clip_grad_norm_, grad_norm
+        ps = [torch.nn.Parameter(torch.zeros(fi, 64, device=dev)) for _ in range(T)]
+        for p in ps:
+            p.grad = torch.randn(fi, 64, device=dev, generator=g)
+        grads = [p.grad for p in ps]
+        if name == "grad_norm":
+            fn = lambda: grad_norm(grads)  # noqa: E731
+        else:
+            fn = lambda: clip_grad_norm_(ps, 1e-6)  # noqa: E731
+        nbytes = T * fi * 64 * 4 * (1 if name == "grad_norm" else 3)
     elif name == "linear_ce":
         from hackathon_b200.cross_entropy import fused_causal_lm_loss
         h = rnd(T, fi).requires_grad_()

@@ -10,6 +10,13 @@ A drop-in for the Python API of the reference package `solution/` (imoshka2009-l
   cross_entropy.py  fused_causal_lm_loss, FusedLinearCrossEntropy, patch()  chunked linear CE
   fused_ce.py       fused_head_loss, FusedLinearCE, ce_rows                 earlier CE API
 
+Beside them, without a counterpart in the reference:
+
+  logprobs.py       token_logprobs, linear_token_logprobs                   fwd + bwd
+  preference.py     preference_loss                                         fwd + bwd
+  policy.py         policy_loss                                             fwd + bwd
+  grad_norm.py      grad_norm, clip_grad_norm_                              all gradients together
+
 Every op calls hand-written sm_100a kernels through the C-ABI of libqlora_b200.so
 (include/qlora_b200.h); none has a CPU path. `apply()` installs the patches on transformers /
 peft / trl classes, as the reference's apply() does (solution/__init__.py:17-34).

@@ -8,11 +8,16 @@
 //   sequence:  sum_i (sum_t mask L / max(n_i, 1)) / denominator    (default: the rows)
 //
 // The gradient jumps where r crosses a border, so the side is that of the exact l against the
-// border's logarithm B, not of a rounded r. Rounding keeps the order: the fp32 difference says which
-// side it is wherever it is not B's own rounding, and there the 64-bit difference does. k3 cancels for small d: below |d| = 1/2 it is summed
-// as its Taylor series. The forward writes each token's dL/dlogp (fp32, unnormalised) when a
+// border's logarithm B, not of a rounded r. Rounding keeps the order: the fp32 difference says
+// which side it is wherever it is not B's own rounding, and there the 64-bit difference does. k3
+// cancels for small d: below |d| = 1/2 it is summed as its Taylor series. The forward writes each token's dL/dlogp (fp32, unnormalised) when a
 // gradient will be asked for; the backward multiplies it by g and the row's weight. Sums are
 // 64-bit, in a fixed order. Masked places are skipped, whatever they hold.
+//
+// Latency bounds it at the sizes of a batch: forward 4.8 us for 16 x 333 tokens, 6.9 us for 8 x
+// 32768, backward 1.4 and 1.7 us. 512 x 4096 tokens (35 MB with the gradient) take 13.9 us, about
+// 90 instructions a token and two waves of CTAs (16 columns a thread instead of 8 spill registers:
+// 16 us), and 2.9 us backward (5.7 TB/s).
 #include <cmath>
 
 #include "objective.cuh"

@@ -22,6 +22,8 @@ FusedLinearCE) are thin aliases whose `apply` calls these ops.
     linear_ce               per-row CE loss, entropy, argmax of h W^T and the
                             per-row gradient of the loss (logits never whole) dh_rows * g
 
+The post-training ops (token_logprobs, preference, policy) are in objective_ops.py.
+
 No op has a CPU kernel: called on CPU tensors they raise (device_types="cuda").
 """
 

@@ -3,8 +3,8 @@
 u = 2^-24. The preference loss is computed in 64 bits and rounded once: loss and rewards are off by
 u relative (plus the 64-bit sums' own 2^-50 of their terms); a gradient is a coefficient rounded
 to fp32 (u), times g (u), rounded to its type. A policy term is r A with r = e^l in fp32: 4 u for
-the function, u |l| for its argument, 2 u for the products; e^d - d - 1 and e^d - 1 are good to 16 u of
-themselves; the 64-bit sum of the terms is rounded once."""
+the function, u |l| for its argument, 2 u for the products; e^d - d - 1 and e^d - 1 are good to
+16 u of themselves; the 64-bit sum of the terms is rounded once."""
 
 import math
 
