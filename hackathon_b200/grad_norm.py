@@ -99,7 +99,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     min(1, max_norm / (norm + 1e-6)) and returns their norm before that, as grad_norm does.
     Parameters without a gradient are left out. An infinite or NaN norm spreads into the
     gradients, unless error_if_nonfinite raises before anything is scaled (a host read).
-    Gradients that share memory are refused."""
+    Gradients that share memory are refused (those with gaps between their elements are scaled
+    through a copy and written back, and not looked at for that)."""
     order = _order("clip_grad_norm_", norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

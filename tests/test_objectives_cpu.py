@@ -306,3 +306,44 @@ def test_dense_layouts_are_recognised():
         assert _fills_its_memory(t)
     for t in (x[:, :5], x[..., ::2], x[0, :1].expand(3, 5), x.unfold(2, 3, 1)):
         assert not _fills_its_memory(t)
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """A call for another device than the current one makes it the current one and passes its
+    stream; a failing call raises the library's message either way."""
+    entered, seen = [], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *exc):
+            entered.append(None)
+
+    class Lib:
+        status = 0
+
+        def qb_thing(self, *args):
+            seen.append((args, list(entered)))
+            return self.status
+
+        def qb_last_error(self):
+            return b"the reason"
+
+    lib = Lib()
+    monkeypatch.setattr(_lib, "_lib", lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    _lib.call_on(torch.device("cuda", 0), "qb_thing", 5)
+    _lib.call_on(torch.device("cuda"), "qb_thing", 6)
+    _lib.call_on(torch.device("cuda", 1), "qb_thing", 7)
+    assert seen == [((5, 100), []), ((6, 100), []), ((7, 101), [1])] and entered == [1, None]
+    lib.status = 1
+    for index in (0, 1):
+        with pytest.raises(RuntimeError, match="qb_thing failed .status 1.: the reason"):
+            _lib.call_on(torch.device("cuda", index), "qb_thing")
+    assert entered == [1, None, 1, None]

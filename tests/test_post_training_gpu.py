@@ -248,3 +248,76 @@ def test_materialised_logits_to_clipped_head(cuda):
     t.copy_(torch.randint(0, 500, t.shape, device=cuda, generator=g))
     graph.replay()
     check(total, norm)
+
+
+def test_two_threads_at_once(cuda):
+    """The operators hold nothing between calls: two threads on two streams get the bits of one."""
+    import threading
+
+    from hackathon_b200.grad_norm import clip_grad_norm_
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+
+    def chain(seed):
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        z = torch.randn(4, 40, 3001, device=cuda, generator=g).requires_grad_()
+        t = torch.randint(0, 3001, (4, 40), device=cuda, generator=g)
+        adv = torch.randn(4, device=cuda, generator=g)
+        lp, en = token_logprobs(z, t, 0.8, True)
+        loss = policy_loss(lp, lp.detach() * 1.01, adv)[0] + preference_loss(lp)[0] - en.mean()
+        loss.backward()
+        norm = clip_grad_norm_(z, 1e-3)
+        return [loss.detach(), norm, z.grad]
+
+    want = [chain(0), chain(1)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = chain(k)
+                stream.synchronize()
+                if not all(map(torch.equal, got, want[k])):
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+def test_inference_mode_checkpoints_and_changed_inputs(cuda):
+    """Inference mode gives the same values; a recomputing checkpoint the same gradients; logits
+    changed between forward and backward are an error, not another gradient."""
+    from torch.utils.checkpoint import checkpoint
+
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.policy import policy_loss
+    g = torch.Generator(device=cuda).manual_seed(3)
+    z = torch.randn(3, 20, 777, device=cuda, generator=g).requires_grad_()
+    t = torch.randint(0, 777, (3, 20), device=cuda, generator=g)
+    adv = torch.randn(3, device=cuda, generator=g)
+
+    def loss_of(logits):
+        lp = token_logprobs(logits, t)
+        return policy_loss(lp, lp.detach() - 0.1, adv)[0]
+
+    with torch.inference_mode():
+        quiet = loss_of(z)
+    loss = loss_of(z)
+    assert torch.equal(quiet, loss.detach())
+    (want,) = torch.autograd.grad(loss, z)
+    (got,) = torch.autograd.grad(checkpoint(loss_of, z, use_reentrant=False), z)
+    assert torch.equal(got, want)
+    x = z.detach() * 1.0
+    leaf = x.requires_grad_()
+    loss = loss_of(leaf)
+    with torch.no_grad():
+        leaf.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
