@@ -33,10 +33,21 @@ _ops = getattr(torch.ops, NS)
 _below_autograd = torch._C._AutoDispatchBelowAutograd
 
 
+def _plain(t):
+    """A tensor the dispatcher would hand to the CUDA kernel as it is: no subclass (fake and
+    functional tensors are), no mode that wants to see the op."""
+    return type(t) in _PLAIN and t.is_cuda and torch._C._len_torch_dispatch_stack() == 0
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
 def _register(schema, fake, function=None):
     """Registers the decorated function as the CUDA kernel of the op `schema` declares, with its
-    fake implementation; `function`: the autograd.Function that calls it when the first argument
-    asks for a gradient. Returns what calls the op."""
+    fake implementation; `function`: the autograd.Function that runs it when the first argument
+    asks for a gradient. Returns what calls the op, with .below for the call below autograd. On
+    plain CUDA tensors (_plain of the first argument) both go to the kernel without the
+    dispatcher, whose boxing of the arguments took 5 to 9 us of a call."""
     name = schema[:schema.index("(")]
 
     def register(kernel):
@@ -44,20 +55,43 @@ def _register(schema, fake, function=None):
         _library.impl(name, kernel, "CUDA")
         torch.library.register_fake(f"{NS}::{name}", fake, lib=_library)
         op = getattr(_ops, name).default
-        if function is None:
-            return op
 
-        def autograd(*args):
-            if torch.is_grad_enabled() and args[0].requires_grad:
-                return function.apply(*args)
+        def below(*args):
+            if _plain(args[0]):
+                return kernel(*args)
             with _below_autograd():
                 return op(*args)
-        _library.impl(name, autograd, "Autograd")
 
-        def call(*args):    # what the op does first, without the way through the dispatcher
+        def autograd(*args):
+            if function is not None and torch.is_grad_enabled() and args[0].requires_grad:
+                return function.apply(*args)
+            return below(*args)
+
+        def call(*args):
             return op(*args) if torch.compiler.is_compiling() else autograd(*args)
+
+        if function is not None:
+            _library.impl(name, autograd, "Autograd")
+        call.below = below
         return call
     return register
+
+
+def _need(ok, op, what):
+    """The kernels read raw addresses: what an op's caller passes has to be what they read."""
+    if not ok:
+        raise ValueError(f"qlora_b200::{op}: {what}")
+
+
+def _mask_fits(mask, shape):
+    return mask is None or _fits(mask, torch.uint8 if mask.dtype == torch.uint8 else torch.bool,
+                                 shape)
+
+
+def _fits(t, dtype, shape):
+    """None, or a contiguous CUDA tensor of this dtype and shape."""
+    return t is None or (t.is_cuda and t.dtype == dtype and t.shape == shape
+                         and t.is_contiguous())
 
 
 class PreferenceConfig(ctypes.Structure):
@@ -97,9 +131,7 @@ def row_layout(logits):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, temperature, with_entropy):
-        with _below_autograd():
-            logp, entropy, state = _ops.token_logprobs.default(logits, target, temperature,
-                                                               with_entropy)
+        logp, entropy, state = token_logprobs.below(logits, target, temperature, with_entropy)
         ctx.save_for_backward(logits, target, state, entropy if with_entropy else None)
         ctx.temperature, ctx.with_entropy = temperature, with_entropy
         ctx.set_materialize_grads(False)
@@ -146,6 +178,8 @@ def _token_logprobs_fake(logits, target, temperature, with_entropy):
 @_register("token_logprobs(Tensor logits, Tensor target, float temperature, bool with_entropy) "
            "-> (Tensor, Tensor, Tensor)", _token_logprobs_fake, _TokenLogprobs)
 def token_logprobs(logits, target, temperature, with_entropy):
+    _need(target.is_cuda and target.dtype == torch.int64 and target.shape == logits.shape[:-1],
+          "token_logprobs", "target is an int64 CUDA tensor of the logits' leading shape")
     z, rows, inner, so, si = row_layout(logits)
     vocab, dev = logits.shape[-1], logits.device
     logp = torch.empty(target.shape, dtype=F32, device=dev)
@@ -166,6 +200,13 @@ def token_logprobs(logits, target, temperature, with_entropy):
            "Tensor? g_logp, Tensor? g_entropy, float temperature) -> Tensor",
            lambda logits, *_: logits.new_empty(logits.shape))
 def token_logprobs_bwd(logits, target, state, entropy, g_logp, g_entropy, temperature):
+    shape = logits.shape[:-1]
+    _need(target.is_cuda and target.dtype == torch.int64 and target.shape == shape
+          and state.is_cuda and state.dtype == F32 and state.is_contiguous()
+          and state.numel() >= 2 * target.numel() and _fits(entropy, F32, shape)
+          and all(g is None or (g.is_cuda and g.dtype == F32 and g.shape == shape)
+                  for g in (g_logp, g_entropy)),
+          "token_logprobs_bwd", "target, state, entropy and gradients as the forward has them")
     z, rows, inner, so, si = row_layout(logits)
     vocab, dev = logits.shape[-1], logits.device
     out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
@@ -187,8 +228,7 @@ def token_logprobs_bwd(logits, target, state, entropy, g_logp, g_entropy, temper
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, mask, *args):
-        with _below_autograd():
-            loss, state = _ops.preference.default(logp, mask, *args)
+        loss, state = preference.below(logp, mask, *args)
         ctx.save_for_backward(mask, state)
         ctx.shape, ctx.dtype, ctx.args = logp.shape, logp.dtype, len(args)
         ctx.set_materialize_grads(False)
@@ -202,7 +242,7 @@ class _Preference(torch.autograd.Function):
         none = (None,) * (ctx.args + 1)
         if g is None:
             return None, *none
-        return preference_bwd(mask, state, g, *ctx.shape, ctx.dtype), *none
+        return preference_bwd(state, mask, g, *ctx.shape, ctx.dtype), *none
 
 
 def preference_state(n, cols):
@@ -225,6 +265,11 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
                loss_type, length_normalized):
     n, cols = logp.shape
     dev = logp.device
+    _need(logp.is_contiguous() and _fits(ref, logp.dtype, logp.shape)
+          and _fits(ref_row, F32, (n,)) and _fits(denominator, torch.float64, ())
+          and _mask_fits(mask, logp.shape), "preference",
+          "contiguous CUDA tensors: ref in logp's dtype, ref_row fp32, bool or byte mask, double "
+          "denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = preference_state(n, cols)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -240,10 +285,13 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
     return loss, state
 
 
-@_register("preference_bwd(Tensor? mask, Tensor state, Tensor g, SymInt n, SymInt cols, "
+@_register("preference_bwd(Tensor state, Tensor? mask, Tensor g, SymInt n, SymInt cols, "
            "ScalarType dtype) -> Tensor",
-           lambda mask, state, g, n, cols, dtype: state.new_empty((n, cols), dtype=dtype))
-def preference_bwd(mask, state, g, n, cols, dtype):
+           lambda state, mask, g, n, cols, dtype: state.new_empty((n, cols), dtype=dtype))
+def preference_bwd(state, mask, g, n, cols, dtype):
+    _need(state.is_cuda and state.dtype == F32 and state.is_contiguous()
+          and state.numel() >= 2 * n and _fits(g, F32, ()) and _mask_fits(mask, (n, cols)),
+          "preference_bwd", "state, mask and gradient as the forward has them")
     out = torch.empty((n, cols), dtype=dtype, device=state.device)
     _lib.call_on(state.device, "qb_preference_bwd", _lib.ptr(mask), state.data_ptr() + 4 * n,
                  g.data_ptr(), n // 2, cols, out.data_ptr(), _lib.tag(dtype),
@@ -258,8 +306,7 @@ def preference_bwd(mask, state, g, n, cols, dtype):
 class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, *args):
-        with _below_autograd():
-            loss, state, unit = _ops.policy.default(logp, *args)
+        loss, state, unit = policy.below(logp, *args)
         ctx.save_for_backward(state, unit)
         ctx.dtype, ctx.args, ctx.sequence, ctx.with_grad = logp.dtype, len(args), *args[-2:]
         ctx.set_materialize_grads(False)
@@ -302,6 +349,12 @@ def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_hi
            kl_coef, divide_by, sequence, with_grad):
     n, cols = logp.shape
     dev = logp.device
+    _need(logp.is_contiguous() and _fits(old_logp, logp.dtype, logp.shape)
+          and _fits(ref, logp.dtype, logp.shape) and _mask_fits(mask, logp.shape)
+          and _fits(denominator, torch.float64, ()) and advantages.is_cuda
+          and advantages.dtype == F32 and advantages.shape in ((n,), (n, cols)), "policy",
+          "contiguous CUDA tensors: old_logp and ref in logp's dtype, fp32 advantages, bool or "
+          "byte mask, double denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = policy_state(n, cols, sequence)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -325,6 +378,10 @@ def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_hi
            lambda unit, state, g, sequence, dtype: unit.new_empty(unit.shape, dtype=dtype))
 def policy_bwd(unit, state, g, sequence, dtype):
     n, cols = unit.shape
+    _need(unit.is_cuda and unit.dtype == F32 and unit.is_contiguous() and _fits(g, F32, ())
+          and state.is_cuda and state.dtype == F32 and state.is_contiguous()
+          and state.numel() >= 4 + (n if sequence else 1), "policy_bwd",
+          "unit gradient, state and gradient as the forward has them")
     out = torch.empty((n, cols), dtype=dtype, device=unit.device)
     _lib.call_on(unit.device, "qb_policy_bwd", unit.data_ptr(), state.data_ptr() + 16,
                  int(sequence), g.data_ptr(), n, cols, out.data_ptr(), _lib.tag(dtype),

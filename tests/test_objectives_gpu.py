@@ -507,6 +507,52 @@ def test_strided_log_probabilities(cuda):
     assert not base.grad[:, -1].any() and base.grad[:, :-1].any()
 
 
+def test_ops_refuse_what_their_kernels_do_not_read(cuda):
+    """Direct calls of the ops with tensors of another device, dtype, shape or layout."""
+    logp, mask, randn = draw(cuda, 4, 30, torch.float32, 91)
+    z, t = randn(4, 90), torch.tensor([3, -100, 5, 89], device=cuda)
+    ns = torch.ops.qlora_b200
+    g, adv = torch.ones((), device=cuda), randn(4)
+    lp, en, state = ns.token_logprobs(z, t, 0.9, True)
+    for bad in (t.cpu(), t.int(), t[:3], t[None]):
+        with pytest.raises(ValueError, match="token_logprobs"):
+            ns.token_logprobs(z, bad, 0.9, True)
+    good = [z, t, state, en, lp, en, 0.9]
+    for k, bad in ((1, t.cpu()), (2, state[:4]), (2, state.double()), (3, en[:2]), (3, en.cpu()),
+                   (4, lp.double()), (4, lp.cpu()), (5, en[:3])):
+        with pytest.raises(ValueError, match="token_logprobs_bwd"):
+            ns.token_logprobs_bwd(*good[:k], bad, *good[k + 1:])
+
+    def pref(x=logp, m=mask, ref=None, row=None, denom=None):
+        return ns.preference(x, m, ref, row, denom, 0.1, 0.0, 0.0, 0.0, 0, False)
+
+    pstate = pref()[1]
+    for bad in (dict(x=logp.t()), dict(m=mask.cpu()), dict(m=mask[:2]), dict(m=mask.float()),
+                dict(m=mask.t().contiguous().t()), dict(ref=logp.half()), dict(ref=logp.cpu()),
+                dict(row=adv.double()), dict(row=adv[:2]), dict(denom=g),
+                dict(denom=g.double().cpu())):
+        with pytest.raises(ValueError, match="preference"):
+            pref(**bad)
+    for bad in ((pstate[:4], mask, g), (pstate, mask[:2], g), (pstate, mask, g.double()),
+                (pstate, mask, g.cpu()), (pstate.cpu(), mask, g)):
+        with pytest.raises((ValueError, NotImplementedError)):
+            ns.preference_bwd(*bad, 4, 30, torch.float32)
+
+    def pol(x=logp, old=logp, a=adv, m=mask, ref=None, denom=None):
+        return ns.policy(x, old, a, m, ref, denom, 0.2, 0.2, 0.0, 0.0, 0.0, True, True)
+
+    _, lstate, unit = pol()
+    for bad in (dict(x=logp.t()), dict(old=logp.half()), dict(old=logp[:2]), dict(a=adv.double()),
+                dict(a=adv[:2]), dict(a=adv.cpu()), dict(m=mask.cpu()), dict(ref=logp[:, :4]),
+                dict(denom=g)):
+        with pytest.raises(ValueError, match="policy"):
+            pol(**bad)
+    for bad in ((unit.double(), lstate, g), (unit, lstate[:6], g), (unit, lstate, g.double()),
+                (unit, lstate.cpu(), g), (unit.t(), lstate, g)):
+        with pytest.raises(ValueError, match="policy_bwd"):
+            ns.policy_bwd(*bad, True, torch.float32)
+
+
 NAMES = ("token_logprobs", "token_logprobs_bwd", "preference", "preference_bwd", "policy",
          "policy_bwd")
 
@@ -524,7 +570,7 @@ def test_opcheck(cuda, name):
     args = {"token_logprobs": (z.requires_grad_(), t, 0.9, True),
             "token_logprobs_bwd": (z.detach(), t, stats, en, lp, en, 0.9),
             "preference": (logp.clone().requires_grad_(), *pref[1:]),
-            "preference_bwd": (mask, oo.preference(*pref)[1], g, 4, 30, torch.bfloat16),
+            "preference_bwd": (oo.preference(*pref)[1], mask, g, 4, 30, torch.bfloat16),
             "policy": (logp.clone().requires_grad_(), *pol[1:]),
             "policy_bwd": (oo.policy(*pol)[2], oo.policy(*pol)[1], g, True, torch.float32)}[name]
     # the objectives' second output ends in workspace, which no two runs fill alike in the same
