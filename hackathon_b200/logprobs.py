@@ -42,7 +42,13 @@ def linear_token_logprobs(hidden, weight, target, chunk_rows=CHUNK_ROWS):
     """(ln softmax(hidden @ weight.T)[target], entropy) per position, fp32, without the logits:
     the linear cross-entropy's kernels, whose per-token loss is the negative log-probability. The
     log-probability is differentiable in the hidden states; the entropy is a constant and the
-    head is frozen. A target of IGNORE_INDEX scores 0."""
+    head is frozen. hidden [..., H], weight [V, H], target [...]; a target of IGNORE_INDEX scores
+    0."""
+    _lib.require_cuda(hidden, weight, target, what="linear_token_logprobs")
+    if (hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]
+            or target.shape != hidden.shape[:-1]):
+        raise ValueError(f"linear_token_logprobs: hidden {tuple(hidden.shape)} and weight "
+                         f"{tuple(weight.shape)} for target {tuple(target.shape)}")
     matmul_dtype = _common.autocast_dtype() or torch.promote_types(hidden.dtype, weight.dtype)
     _, token_loss, entropy, _ = FusedLinearCrossEntropy.apply(hidden, weight, target, 1,
                                                               matmul_dtype, chunk_rows)

@@ -83,15 +83,15 @@ def _need(ok, op, what):
         raise ValueError(f"qlora_b200::{op}: {what}")
 
 
-def _mask_fits(mask, shape):
-    return mask is None or _fits(mask, torch.uint8 if mask.dtype == torch.uint8 else torch.bool,
-                                 shape)
-
-
-def _fits(t, dtype, shape):
-    """None, or a contiguous CUDA tensor of this dtype and shape."""
-    return t is None or (t.is_cuda and t.dtype == dtype and t.shape == shape
+def _fits(t, at, dtype, shape):
+    """None, or a contiguous tensor of this dtype and shape on the CUDA device numbered `at`."""
+    return t is None or (t.get_device() == at and t.dtype == dtype and t.shape == shape
                          and t.is_contiguous())
+
+
+def _mask_fits(mask, at, shape):
+    return mask is None or _fits(mask, at,
+                                 torch.uint8 if mask.dtype == torch.uint8 else torch.bool, shape)
 
 
 class PreferenceConfig(ctypes.Structure):
@@ -178,8 +178,9 @@ def _token_logprobs_fake(logits, target, temperature, with_entropy):
 @_register("token_logprobs(Tensor logits, Tensor target, float temperature, bool with_entropy) "
            "-> (Tensor, Tensor, Tensor)", _token_logprobs_fake, _TokenLogprobs)
 def token_logprobs(logits, target, temperature, with_entropy):
-    _need(target.is_cuda and target.dtype == torch.int64 and target.shape == logits.shape[:-1],
-          "token_logprobs", "target is an int64 CUDA tensor of the logits' leading shape")
+    _need(target.get_device() == logits.get_device() and target.dtype == torch.int64
+          and target.shape == logits.shape[:-1], "token_logprobs",
+          "target is an int64 tensor of the logits' leading shape on their device")
     z, rows, inner, so, si = row_layout(logits)
     vocab, dev = logits.shape[-1], logits.device
     logp = torch.empty(target.shape, dtype=F32, device=dev)
@@ -200,11 +201,11 @@ def token_logprobs(logits, target, temperature, with_entropy):
            "Tensor? g_logp, Tensor? g_entropy, float temperature) -> Tensor",
            lambda logits, *_: logits.new_empty(logits.shape))
 def token_logprobs_bwd(logits, target, state, entropy, g_logp, g_entropy, temperature):
-    shape = logits.shape[:-1]
-    _need(target.is_cuda and target.dtype == torch.int64 and target.shape == shape
-          and state.is_cuda and state.dtype == F32 and state.is_contiguous()
-          and state.numel() >= 2 * target.numel() and _fits(entropy, F32, shape)
-          and all(g is None or (g.is_cuda and g.dtype == F32 and g.shape == shape)
+    shape, at = logits.shape[:-1], logits.get_device()
+    _need(target.get_device() == at and target.dtype == torch.int64 and target.shape == shape
+          and state.get_device() == at and state.dtype == F32 and state.is_contiguous()
+          and state.numel() >= 2 * target.numel() and _fits(entropy, at, F32, shape)
+          and all(g is None or (g.get_device() == at and g.dtype == F32 and g.shape == shape)
                   for g in (g_logp, g_entropy)),
           "token_logprobs_bwd", "target, state, entropy and gradients as the forward has them")
     z, rows, inner, so, si = row_layout(logits)
@@ -265,11 +266,12 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
                loss_type, length_normalized):
     n, cols = logp.shape
     dev = logp.device
-    _need(logp.is_contiguous() and _fits(ref, logp.dtype, logp.shape)
-          and _fits(ref_row, F32, (n,)) and _fits(denominator, torch.float64, ())
-          and _mask_fits(mask, logp.shape), "preference",
-          "contiguous CUDA tensors: ref in logp's dtype, ref_row fp32, bool or byte mask, double "
-          "denominator")
+    here = logp.get_device()
+    _need(logp.is_contiguous() and _fits(ref, here, logp.dtype, logp.shape)
+          and _fits(ref_row, here, F32, (n,)) and _fits(denominator, here, torch.float64, ())
+          and _mask_fits(mask, here, logp.shape), "preference",
+          "contiguous tensors on one device: ref in logp's dtype, ref_row fp32, bool or byte mask, "
+          "double denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = preference_state(n, cols)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -289,8 +291,9 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
            "ScalarType dtype) -> Tensor",
            lambda state, mask, g, n, cols, dtype: state.new_empty((n, cols), dtype=dtype))
 def preference_bwd(state, mask, g, n, cols, dtype):
-    _need(state.is_cuda and state.dtype == F32 and state.is_contiguous()
-          and state.numel() >= 2 * n and _fits(g, F32, ()) and _mask_fits(mask, (n, cols)),
+    here = state.get_device()
+    _need(state.dtype == F32 and state.is_contiguous() and state.numel() >= 2 * n
+          and _fits(g, here, F32, ()) and _mask_fits(mask, here, (n, cols)),
           "preference_bwd", "state, mask and gradient as the forward has them")
     out = torch.empty((n, cols), dtype=dtype, device=state.device)
     _lib.call_on(state.device, "qb_preference_bwd", _lib.ptr(mask), state.data_ptr() + 4 * n,
@@ -349,12 +352,14 @@ def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_hi
            kl_coef, divide_by, sequence, with_grad):
     n, cols = logp.shape
     dev = logp.device
-    _need(logp.is_contiguous() and _fits(old_logp, logp.dtype, logp.shape)
-          and _fits(ref, logp.dtype, logp.shape) and _mask_fits(mask, logp.shape)
-          and _fits(denominator, torch.float64, ()) and advantages.is_cuda
-          and advantages.dtype == F32 and advantages.shape in ((n,), (n, cols)), "policy",
-          "contiguous CUDA tensors: old_logp and ref in logp's dtype, fp32 advantages, bool or "
-          "byte mask, double denominator")
+    here = logp.get_device()
+    _need(logp.is_contiguous() and _fits(old_logp, here, logp.dtype, logp.shape)
+          and _fits(ref, here, logp.dtype, logp.shape) and _mask_fits(mask, here, logp.shape)
+          and _fits(denominator, here, torch.float64, ())
+          and advantages.get_device() == here and advantages.dtype == F32
+          and advantages.shape in ((n,), (n, cols)), "policy",
+          "contiguous tensors on one device: old_logp and ref in logp's dtype, fp32 advantages, "
+          "bool or byte mask, double denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = policy_state(n, cols, sequence)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -378,8 +383,9 @@ def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_hi
            lambda unit, state, g, sequence, dtype: unit.new_empty(unit.shape, dtype=dtype))
 def policy_bwd(unit, state, g, sequence, dtype):
     n, cols = unit.shape
-    _need(unit.is_cuda and unit.dtype == F32 and unit.is_contiguous() and _fits(g, F32, ())
-          and state.is_cuda and state.dtype == F32 and state.is_contiguous()
+    here = unit.get_device()
+    _need(unit.dtype == F32 and unit.is_contiguous() and _fits(g, here, F32, ())
+          and state.get_device() == here and state.dtype == F32 and state.is_contiguous()
           and state.numel() >= 4 + (n if sequence else 1), "policy_bwd",
           "unit gradient, state and gradient as the forward has them")
     out = torch.empty((n, cols), dtype=dtype, device=unit.device)

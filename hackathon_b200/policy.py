@@ -14,23 +14,23 @@ class PolicyStep:
     the lower and the upper border of the ratio hold."""
 
     def __init__(self, state):
-        self.stats = state          # the op's second output: the statistics come first
+        self.state = state          # the op's second output: the statistics come first
 
     @property
     def tokens(self):
-        return self.stats[0]
+        return self.state[0]
 
     @property
     def kl(self):
-        return self.stats[1]
+        return self.state[1]
 
     @property
     def clipped_low(self):
-        return self.stats[2]
+        return self.state[2]
 
     @property
     def clipped_high(self):
-        return self.stats[3]
+        return self.state[3]
 
 
 def policy_loss(logp, old_logp, advantages, mask=None, ref_logp=None, clip_low=0.2,

@@ -218,6 +218,10 @@ def test_token_logprobs_refusals():
         for bad in (0.0, -1.0, math.nan, math.inf):
             with pytest.raises(ValueError, match="temperature"):
                 token_logprobs(e(2, 5, 30), t, bad)
+        for h, w, target in ((e(2, 5, 8), e(30, 8), t[:, :4]), (e(2, 5, 8), e(30, 9), t),
+                             (e(2, 5, 8), e(8), t), (e(2, 5, 8), e(30, 8), t.reshape(10))):
+            with pytest.raises(ValueError, match="linear_token_logprobs"):
+                linear_token_logprobs(h, w, target)
     _fake_cuda(run)
     with pytest.raises(RuntimeError, match="CUDA"):
         linear_token_logprobs(torch.ones(2, 8), torch.ones(10, 8), torch.ones(2, dtype=I64))

@@ -308,7 +308,7 @@ def test_policy_masked_places_may_hold_anything(cuda):
                                      reduction=reduction)
             (g,) = torch.autograd.grad(loss, x)
             assert torch.equal(loss, want) and torch.isfinite(g).all() and not g[~mask].any()
-            assert torch.isfinite(step.stats[:4]).all()
+            assert torch.isfinite(step.state[:4]).all()
         none = torch.zeros_like(mask)
         x = logp.detach().requires_grad_()
         loss, step = policy_loss(x, old, adv, none, ref, kl_coef=0.1, reduction=reduction)
