@@ -101,7 +101,7 @@ __device__ __forceinline__ H2 word_as(uint32_t w) {
   memcpy(&h, &w, 4);
   return h;
 }
-template <typename T, typename H2> struct Vec16Bit {
+template <typename H2> struct Vec16Bit {
   static constexpr int N = 8;
   uint4 u;
   __device__ __forceinline__ uint32_t word(int k) const {
@@ -115,7 +115,7 @@ template <typename T, typename H2> struct Vec16Bit {
     return max_nan(qb::to_f(m.x), qb::to_f(m.y));
   }
 };
-template <> struct Vec<__nv_bfloat16> : Vec16Bit<__nv_bfloat16, __nv_bfloat162> {
+template <> struct Vec<__nv_bfloat16> : Vec16Bit<__nv_bfloat162> {
   __device__ __forceinline__ Pair less(int k, float m) const {
     float lo, hi;
     asm("add.rn.f32.bf16 %0, %1, %2;" : "=f"(lo) : "h"(low(k)), "f"(-m));
@@ -124,7 +124,7 @@ template <> struct Vec<__nv_bfloat16> : Vec16Bit<__nv_bfloat16, __nv_bfloat162> 
   }
   static __device__ __forceinline__ uint32_t none() { return 0xff80ff80u; }
 };
-template <> struct Vec<__half> : Vec16Bit<__half, __half2> {
+template <> struct Vec<__half> : Vec16Bit<__half2> {
   __device__ __forceinline__ Pair less(int k, float m) const {
     float lo, hi;
     asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(lo) : "h"(low(k)), "f"(-m));
