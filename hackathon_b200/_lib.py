@@ -86,7 +86,7 @@ _SIGNATURES = {
                               _p, _p],
     "qb_preference_config_size": [],
     "qb_preference_workspace": [_i64, _i64],
-    "qb_preference_fwd": [_p, _p, _i32, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p],
+    "qb_preference_fwd": [_p, _p, _i32, _p, _p, _i32, _i64, _i64, _p, _p, _p, _p, _p, _p, _p],
     "qb_preference_bwd": [_p, _p, _p, _i64, _i64, _p, _i32, _p],
     "qb_policy_config_size": [],
     "qb_policy_workspace": [_i64, _i64],

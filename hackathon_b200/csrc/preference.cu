@@ -72,9 +72,10 @@ __device__ double sigmoid(double x) {
 // One CTA: a group of lanes per pair, the rows' records added in a fixed order.
 __global__ void __launch_bounds__(1024)
 preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lanes, int64_t pairs,
-                        const float* __restrict__ ref_row, qb_preference_config cfg,
-                        const double* __restrict__ denom_dev, float* __restrict__ loss,
-                        float* __restrict__ rewards, float* __restrict__ coef) {
+                        const void* __restrict__ ref_row, bool ref_row_double,
+                        qb_preference_config cfg, const double* __restrict__ denom_dev,
+                        float* __restrict__ loss, float* __restrict__ rewards,
+                        float* __restrict__ coef) {
   qb::await_previous();
   __shared__ double scratch[32];
   const double denom = denom_dev ? *denom_dev
@@ -104,7 +105,9 @@ preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lane
     for (int h = 0; h < 2; ++h) {
       const int64_t row = p + h * pairs;
       n[h] = cfg.length_normalized ? fmax(n[h], 1.0) : 1.0;
-      s[h] = s[h] / n[h] - (ref_row ? double(ref_row[row]) : 0.0);
+      s[h] = s[h] / n[h] - (!ref_row ? 0.0
+                            : ref_row_double ? static_cast<const double*>(ref_row)[row]
+                                             : static_cast<const float*>(ref_row)[row]);
       rewards[row] = static_cast<float>(cfg.beta * s[h]);
     }
     const double d = s[0] - s[1], u = cfg.beta * d - cfg.margin;
@@ -168,8 +171,8 @@ extern "C" int64_t qb_preference_workspace(int64_t pairs, int64_t cols) {
 }
 
 extern "C" int qb_preference_fwd(const void* logp, const void* ref, int dtype,
-                                 const uint8_t* mask, const float* ref_row, int64_t pairs,
-                                 int64_t cols, const qb_preference_config* cfg,
+                                 const uint8_t* mask, const void* ref_row, int ref_row_double,
+                                 int64_t pairs, int64_t cols, const qb_preference_config* cfg,
                                  const double* denominator, float* loss, float* rewards,
                                  float* coef, void* workspace, cudaStream_t stream) {
   if (int rc = check("preference", pairs, cols)) return rc;
@@ -189,7 +192,8 @@ extern "C" int qb_preference_fwd(const void* logp, const void* ref, int dtype,
   if (int rc = qb::check_launch("preference")) return rc;
   const int lanes = qb::lanes_per_row(chunks);
   qb::launch_after(preference_pairs_kernel, 1, qb::adding_threads(pairs, lanes), stream, records,
-                   chunks, lanes, pairs, ref_row, *cfg, denominator, loss, rewards, coef);
+                   chunks, lanes, pairs, ref_row, ref_row_double != 0, *cfg, denominator, loss,
+                   rewards, coef);
   return qb::check_launch("preference");
 }
 

@@ -27,7 +27,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .ops import NS
 
-F32 = torch.float32
+F32, F64 = torch.float32, torch.float64
 _library = torch.library.Library(NS, "FRAGMENT")
 _ops = getattr(torch.ops, NS)
 _below_autograd = torch._C._AutoDispatchBelowAutograd
@@ -268,10 +268,12 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
     dev = logp.device
     here = logp.get_device()
     _need(logp.is_contiguous() and _fits(ref, here, logp.dtype, logp.shape)
-          and _fits(ref_row, here, F32, (n,)) and _fits(denominator, here, torch.float64, ())
+          and (ref_row is None or ref_row.dtype in (F32, F64)
+               and _fits(ref_row, here, ref_row.dtype, (n,)))
+          and _fits(denominator, here, F64, ())
           and _mask_fits(mask, here, logp.shape), "preference",
-          "contiguous tensors on one device: ref in logp's dtype, ref_row fp32, bool or byte mask, "
-          "double denominator")
+          "contiguous tensors on one device: ref in logp's dtype, ref_row fp32 or fp64, bool or "
+          "byte mask, double denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = preference_state(n, cols)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -280,7 +282,9 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
                            length_normalized)
     e = logp.element_size()
     _lib.call_on(dev, "qb_preference_fwd", logp.data_ptr(), _lib.ptr(ref), _lib.tag(logp.dtype),
-                 _lib.ptr(mask), _lib.ptr(ref_row), n // 2, cols, ctypes.addressof(cfg),
+                 _lib.ptr(mask), _lib.ptr(ref_row),
+                 int(ref_row is not None and ref_row.dtype == F64), n // 2, cols,
+                 ctypes.addressof(cfg),
                  _lib.ptr(denominator), loss.data_ptr(), base, base + 4 * n, base + 4 * at,
                  kernels=2,
                  work=(n * cols * (e * (1 if ref is None else 2) + (mask is not None)), 0))
@@ -355,7 +359,7 @@ def policy(logp, old_logp, advantages, mask, ref, denominator, clip_low, clip_hi
     here = logp.get_device()
     _need(logp.is_contiguous() and _fits(old_logp, here, logp.dtype, logp.shape)
           and _fits(ref, here, logp.dtype, logp.shape) and _mask_fits(mask, here, logp.shape)
-          and _fits(denominator, here, torch.float64, ())
+          and _fits(denominator, here, F64, ())
           and advantages.get_device() == here and advantages.dtype == F32
           and advantages.shape in ((n,), (n, cols)), "policy",
           "contiguous tensors on one device: old_logp and ref in logp's dtype, fp32 advantages, "

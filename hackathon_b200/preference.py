@@ -39,8 +39,8 @@ def preference_loss(logp, mask=None, ref_logp=None, beta=0.1, loss_type="sigmoid
     logp [2P, S] (fp32, fp16 or bf16): rows 0 .. P-1 the preferred sequences, P .. 2P-1 the rejected
     ones of the same pairs. mask [2P, S]: the tokens that count (nonzero; all without one); what
     the others hold is never used. ref_logp: the reference model's, per token [2P, S] or already
-    summed per sequence [2P] (averaged, if length_normalized), or None. With s the masked sum of
-    logp - ref_logp (its mean with length_normalized; 0 for a row without tokens),
+    summed per sequence [2P] (averaged, if length_normalized; fp64 is kept), or None. With s the
+    masked sum of logp - ref_logp (its mean with length_normalized; 0 for a row without tokens),
     D = s_preferred - s_rejected and u = beta * D - margin, a pair's loss is
         sigmoid   -(1 - label_smoothing) * ln sigma(u) - label_smoothing * ln sigma(-u)
         hinge     max(0, 1 - u)
@@ -70,7 +70,8 @@ def preference_loss(logp, mask=None, ref_logp=None, beta=0.1, loss_type="sigmoid
             logp, ref = logp.to(dtype), ref_logp.to(dtype).contiguous()
             _lib.tag(dtype)
         elif ref_logp.shape == (n,):
-            ref_row = ref_logp.to(torch.float32).contiguous()
+            wide = ref_logp.dtype == torch.float64      # long sums keep their 64 bits
+            ref_row = ref_logp.to(torch.float64 if wide else torch.float32).contiguous()
         else:
             raise ValueError(f"preference_loss: ref_logp {tuple(ref_logp.shape)} for logp "
                              f"{tuple(logp.shape)}")

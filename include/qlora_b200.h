@@ -458,9 +458,9 @@ int64_t qb_token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype);
  * (0 for labels outside [0, vocab)), and, when `entropy` is given, the entropy of the row's
  * distribution. Row r of `rows` starts at (r / inner) * stride_outer + (r % inner) *
  * stride_inner elements, so a [batch, positions, vocab] view needs no copy; the last dimension
- * is contiguous. stats [rows, 2] (8-byte aligned) receives (m, sum) for the backward; workspace is 16-byte
- * aligned device memory. Logits of -inf have probability 0; a row of nothing else is NaN. T in
- * 1e-6 .. 1e6. */
+ * is contiguous. stats [rows, 2] (8-byte aligned) receives (m, sum) for the backward; workspace
+ * is 16-byte aligned device memory. Logits of -inf have probability 0; a row of nothing else is
+ * NaN. T in 1e-6 .. 1e6. */
 int qb_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t inner,
                       int64_t stride_outer, int64_t stride_inner, int64_t vocab,
                       const int64_t* target, float temperature, float* logp, float* entropy,
@@ -495,11 +495,11 @@ int64_t qb_preference_workspace(int64_t pairs, int64_t cols);
  *   sigmoid  -(1 - label_smoothing) ln sigma(u) - label_smoothing ln sigma(-u)
  *   hinge    max(0, 1 - u)                     ipo  (D - 1 / (2 beta))^2
  * over the denominator (*denominator, a device double, when given). ref [2 * pairs, cols] in
- * logp's dtype, or ref_row [2 * pairs], or neither; mask bytes [2 * pairs, cols] or NULL (all).
- * rewards [2 * pairs] = beta s; coef [2 * pairs] is what qb_preference_bwd takes. `cfg` is a host
- * pointer; workspace is 16-byte aligned device memory. */
+ * logp's dtype, or ref_row [2 * pairs] (doubles if ref_row_double, else floats), or neither; mask
+ * bytes [2 * pairs, cols] or NULL (all). rewards [2 * pairs] = beta s; coef [2 * pairs] is what
+ * qb_preference_bwd takes. `cfg` is a host pointer; workspace is 16-byte aligned device memory. */
 int qb_preference_fwd(const void* logp, const void* ref, int dtype, const uint8_t* mask,
-                      const float* ref_row, int64_t pairs, int64_t cols,
+                      const void* ref_row, int ref_row_double, int64_t pairs, int64_t cols,
                       const qb_preference_config* cfg, const double* denominator, float* loss,
                       float* rewards, float* coef, void* workspace, cudaStream_t stream);
 

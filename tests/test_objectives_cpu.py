@@ -139,7 +139,7 @@ def test_c_entries_refuse_before_any_launch():
     def pr(cfg=pref, pairs=2, cols=8, ref=None, row=None, logp=fake, **kw):
         keep.append(cfg)               # the call reads it at its address
         at = ctypes.addressof(cfg) if cfg is not None else None
-        return ("qb_preference_fwd", logp, ref, 0, None, row, pairs, cols, at, None, fake, fake,
+        return ("qb_preference_fwd", logp, ref, 0, None, row, 0, pairs, cols, at, None, fake, fake,
                 fake, fake, None)
 
     cases += [(pr(pairs=0), "bad shape"), (pr(cols=0), "bad shape"), (pr(logp=None), "null"),

@@ -162,6 +162,13 @@ def test_long_sums_keep_small_differences(cuda):
     assert abs(got - want) <= 3e5 * 2 * U               # each reward is rounded to fp32
     loss, _ = preference_loss(x, beta=1.0)
     assert abs(float(loss) - math.log1p(math.exp(-want))) <= 2 * U
+    # reference sums in fp64 keep as much: a pair that differs from its reference by 1e-2 each
+    ref = x.double().sum(1) + torch.tensor([1e-2, -1e-2], dtype=torch.float64, device=cuda)
+    loss, step = preference_loss(x, None, ref, beta=1.0)
+    rewards = [float(step.chosen_rewards), float(step.rejected_rewards)]
+    assert abs(rewards[0] + 1e-2) <= 2 * U and abs(rewards[1] - 1e-2) <= 2 * U
+    assert abs(float(loss) - math.log1p(math.exp(2e-2))) <= 2 * U
+    check_preference(x, None, ref, beta=1.0)
 
 
 def test_preference_against_differences(cuda):
@@ -529,7 +536,7 @@ def test_ops_refuse_what_their_kernels_do_not_read(cuda):
     pstate = pref()[1]
     for bad in (dict(x=logp.t()), dict(m=mask.cpu()), dict(m=mask[:2]), dict(m=mask.float()),
                 dict(m=mask.t().contiguous().t()), dict(ref=logp.half()), dict(ref=logp.cpu()),
-                dict(row=adv.double()), dict(row=adv[:2]), dict(denom=g),
+                dict(row=adv.half()), dict(row=adv[:2]), dict(denom=g),
                 dict(denom=g.double().cpu())):
         with pytest.raises(ValueError, match="preference"):
             pref(**bad)
