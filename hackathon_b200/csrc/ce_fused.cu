@@ -9,8 +9,9 @@
 //   reduce  qb_ce_reduce: merges the per-tile partials of every row into lse, loss =
 //           lse - z[label], entropy = lse - t/s, argmax, correct.
 //   pass 2  qb_linear_ce_grad: the logits tile again, epilogue dZ = (e^(z - lse) - onehot) *
-//           scale in bf16 (scale a device scalar, the caller's gradient factor; 0 for unlabelled
-//           rows) — the gradient, not the logits.
+//           scale in bf16 (scale a device scalar, the caller's gradient factor) — the gradient,
+//           not the logits. A row whose target lies outside [0, vocab) is unlabelled in both
+//           passes: loss 0, dZ 0 whatever its logits are.
 //   then    dH = dZ W (qb_gemm_bf16 with W read MN-major), fp32.
 // Executed flops: 3 x 2 N H V against the algorithmic 4 N H V (logits + dH).
 #include <cfloat>
@@ -52,7 +53,8 @@ struct EpiGrad {
     const bool live = r < rows;
     const int64_t label = live ? __ldg(target + r) : -1;
     const float l = live ? __ldg(lse + r) : 0.f;
-    const float sc = (live && label >= 0) ? __ldg(scale_dev) : 0.f;
+    const bool labelled = live && label >= 0 && label < vocab;
+    const float sc = labelled ? __ldg(scale_dev) : 0.f;
     if (lane == 0) tc::bulk_wait_read_all();   // the previous tile's boxes are free
     __syncwarp();
 #pragma unroll 1
@@ -63,7 +65,7 @@ struct EpiGrad {
       if (n >= vocab) continue;   // warp-uniform
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        v[i] = live ? (__expf(v[i] - l) - (n + i == label ? 1.f : 0.f)) * sc : 0.f;
+        v[i] = labelled ? (__expf(v[i] - l) - (n + i == label ? 1.f : 0.f)) * sc : 0.f;
       uint8_t* box = stage + (ch & 1) * kBoxBytes;
       if (ch >= 2) {   // the store of chunk ch - 2 read this box
         if (lane == 0) tc::bulk_wait_read_newest_pending();
@@ -85,7 +87,8 @@ struct EpiGrad {
     const bool live = r < rows;
     const int64_t label = live ? __ldg(target + r) : -1;
     const float l = live ? __ldg(lse + r) : 0.f;
-    const float sc = (live && label >= 0) ? __ldg(scale_dev) : 0.f;
+    const bool labelled = live && label >= 0 && label < vocab;
+    const float sc = labelled ? __ldg(scale_dev) : 0.f;
 #pragma unroll 1
     for (int ch = 0; ch < BN / 32; ++ch) {
       float v[32];
@@ -94,7 +97,7 @@ struct EpiGrad {
       if (!live || n >= vocab) continue;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        v[i] = (__expf(v[i] - l) - (n + i == label ? 1.f : 0.f)) * sc;
+        v[i] = labelled ? (__expf(v[i] - l) - (n + i == label ? 1.f : 0.f)) * sc : 0.f;
       __nv_bfloat16* dst = dz + static_cast<int64_t>(r) * ldz + n;
       if (vec && n + 32 <= vocab) {
 #pragma unroll
@@ -186,9 +189,13 @@ ce_grad_from_logits_kernel(const float* __restrict__ logits, int64_t ldl,
   const int64_t r = blockIdx.x;
   const int64_t label = __ldg(target + r);
   const float l = __ldg(lse + r);
-  const float sc = label >= 0 ? __ldg(scale_dev) : 0.f;
+  const bool labelled = label >= 0 && label < vocab;
+  const float sc = labelled ? __ldg(scale_dev) : 0.f;
   const float* z = logits + r * ldl;
   __nv_bfloat16* d = dz + r * ldz;
+  auto grad = [&](float x, int col) {
+    return labelled ? (__expf(x - l) - (col == label ? 1.f : 0.f)) * sc : 0.f;
+  };
   if (vec) {
     for (int n = threadIdx.x * 8; n < vocab; n += blockDim.x * 8) {
       if (n + 8 <= vocab) {
@@ -196,16 +203,16 @@ ce_grad_from_logits_kernel(const float* __restrict__ logits, int64_t ldl,
         const float4 b = __ldg(reinterpret_cast<const float4*>(z + n + 4));
         float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (__expf(v[i] - l) - (n + i == label ? 1.f : 0.f)) * sc;
+        for (int i = 0; i < 8; ++i) v[i] = grad(v[i], n + i);
         qb::store8<__nv_bfloat16>(d + n, v);
       } else {
         for (int i = n; i < vocab; ++i)
-          d[i] = __float2bfloat16_rn((__expf(z[i] - l) - (i == label ? 1.f : 0.f)) * sc);
+          d[i] = __float2bfloat16_rn(grad(z[i], i));
       }
     }
   } else {
     for (int i = threadIdx.x; i < vocab; i += blockDim.x)
-      d[i] = __float2bfloat16_rn((__expf(z[i] - l) - (i == label ? 1.f : 0.f)) * sc);
+      d[i] = __float2bfloat16_rn(grad(z[i], i));
   }
 }
 

@@ -5,7 +5,8 @@
 // (max m, sum e = exp(z-m), sum e*z, first argmax) over its elements, rescaling once per chunk of
 // 8, and the block merges the partial states. lse = m + log(s), entropy = lse - t/s,
 // loss = lse - z[label] for labelled rows. Pass 2 (write_grad) rewrites the row with
-// (exp(z - lse) - onehot) * scale, scale = grad_scale for labelled rows and 0 otherwise.
+// (exp(z - lse) - onehot) * grad_scale, or with zeros, whatever it holds, when its target lies
+// outside [0, vocab).
 #include <cfloat>
 
 #include "qb_common.cuh"
@@ -117,7 +118,6 @@ ce_rows_kernel(T* __restrict__ logits, int64_t row_stride, const int64_t* __rest
   }
   if (!write_grad) return;
   __syncthreads();  // z[label] is read above before it is overwritten below
-  const float scale = labelled ? grad_scale : 0.f;
   for (int64_t v = threadIdx.x; v < nvec; v += kThreads) {
     float x[VEC];
     if constexpr (VEC == 8) qb::load8<T>(z + v * VEC, x);
@@ -125,14 +125,15 @@ ce_rows_kernel(T* __restrict__ logits, int64_t row_stride, const int64_t* __rest
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const int64_t col = v * VEC + e;
-      x[e] = (__expf(x[e] - lse) - (col == label ? 1.f : 0.f)) * scale;
+      x[e] = labelled ? (__expf(x[e] - lse) - (col == label ? 1.f : 0.f)) * grad_scale : 0.f;
     }
     if constexpr (VEC == 8) qb::store8<T>(z + v * VEC, x);
     else z[v] = qb::from_f<T>(x[0]);
   }
   for (int64_t c = nvec * VEC + threadIdx.x; c < vocab; c += kThreads) {
     const float x = qb::to_f(z[c]);
-    z[c] = qb::from_f<T>((__expf(x - lse) - (c == label ? 1.f : 0.f)) * scale);
+    const float d = labelled ? (__expf(x - lse) - (c == label ? 1.f : 0.f)) * grad_scale : 0.f;
+    z[c] = qb::from_f<T>(d);
   }
 }
 

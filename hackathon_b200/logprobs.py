@@ -42,8 +42,8 @@ def linear_token_logprobs(hidden, weight, target, chunk_rows=CHUNK_ROWS):
     """(ln softmax(hidden @ weight.T)[target], entropy) per position, fp32, without the logits:
     the linear cross-entropy's kernels, whose per-token loss is the negative log-probability. The
     log-probability is differentiable in the hidden states; the entropy is a constant and the
-    head is frozen. hidden [..., H], weight [V, H], target [...]; a target of IGNORE_INDEX scores
-    0."""
+    head is frozen. hidden [..., H], weight [V, H], target [...]; a target outside [0, V)
+    (IGNORE_INDEX) scores 0 and has no gradient."""
     _lib.require_cuda(hidden, weight, target, what="linear_token_logprobs")
     if (hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]
             or target.shape != hidden.shape[:-1]):

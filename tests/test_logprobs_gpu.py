@@ -337,3 +337,37 @@ def test_linear_form_matches_the_materialised_one(cuda, dtype):
     tol = (2 * 2.0 ** -8 if dtype == torch.bfloat16 else 600 * U) * size \
         + 4 * per_logit[..., None] * size
     close(leaf.grad, dz @ w.double(), tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [777, 1000])
+def test_targets_outside_the_vocabulary_score_nothing(cuda, vocab, dtype, monkeypatch):
+    """Any target outside [0, vocab) is a constant 0 with no gradient, as -100 is: the same bits,
+    on the recomputing and on the storing gradient pass, and 0 even from a row of NaN."""
+    from hackathon_b200 import cross_entropy
+    from hackathon_b200.logprobs import linear_token_logprobs
+    g = torch.Generator(device=cuda).manual_seed(vocab)
+    h = torch.randn(150, 256, device=cuda, generator=g).to(dtype)
+    w = (torch.randn(vocab, 256, device=cuda, generator=g) * 0.1).to(dtype)
+    t = torch.randint(0, vocab, (150,), device=cuda, generator=g)
+    out = torch.tensor([vocab, vocab + 5, 1 << 31, 1 << 40, -1, -7, -(1 << 40)], device=cuda)
+    at = torch.arange(3, 3 + 20 * len(out), 20, device=cuda)
+    t[at] = out
+    plain = t.clone()
+    plain[at] = IGNORE
+
+    def run(target, hidden=h):
+        leaf = hidden.detach().requires_grad_()
+        lp, _ = linear_token_logprobs(leaf, w, target)
+        (grad,) = torch.autograd.grad(lp, leaf, torch.linspace(-2, 3, 150, device=cuda))
+        return lp.detach(), grad
+
+    for store in (False, True):
+        monkeypatch.setattr(cross_entropy, "STORE_LOGITS", store)
+        want, got = run(plain), run(t)
+        assert all(map(torch.equal, got, want))
+        assert not got[0][at].any() and not got[1][at].any() and got[1][4].any()
+        broken = h.clone()
+        broken[at] = math.nan
+        lost = run(t, broken)
+        assert torch.equal(lost[0], want[0]) and torch.equal(lost[1], want[1])
