@@ -16,7 +16,7 @@ from dataclasses import dataclass, replace
 import torch
 import torch.nn.functional as F
 
-from .cross_entropy import IGNORE_INDEX, fused_causal_lm_loss, shift_labels_of
+from .cross_entropy import fused_causal_lm_loss, shift_labels_of
 from .grad_norm import clip_grad_norm_
 from .logprobs import linear_token_logprobs
 from .lora import DropoutCast, ScaledAdd
@@ -654,12 +654,12 @@ class QwenQLoRA(torch.nn.Module):
 
     def token_logprobs(self, input_ids, labels):
         """(logp, entropy, mask), each [B, S]: at position t the log-probability of the label at
-        t + 1 (labels shifted as in the loss; 0 where it is -100, and in the last position), the
-        entropy of that prediction, and which positions are scored. The log-probabilities are
-        differentiable in the adapters."""
+        t + 1 (labels shifted as in the loss; 0 where it is no token, as -100 is none, and in the
+        last position), the entropy of that prediction, and which positions are scored. The
+        log-probabilities are differentiable in the adapters."""
         target = shift_labels_of(labels)
         logp, entropy = linear_token_logprobs(self.hidden_states(input_ids), self.lm_head, target)
-        return logp, entropy, target != IGNORE_INDEX
+        return logp, entropy, (target >= 0) & (target < self.lm_head.shape[0])
 
     def hidden_states(self, input_ids):
         """The final norm's output [B, S, hidden]."""

@@ -321,3 +321,26 @@ def test_inference_mode_checkpoints_and_changed_inputs(cuda):
         leaf.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_labels_outside_the_vocabulary_are_not_scored(cuda):
+    """A label of no token takes no part in a step, as -100 takes none."""
+    from hackathon_b200.policy import policy_loss
+    model, shape = tiny()
+    model.train()
+    ids, labels = batch(shape, 4, 64)
+    odd = labels.clone()
+    odd[0, 40:50], odd[2, 60] = shape.vocab, shape.vocab + 9
+    odd[1, 20], plain = -1, labels.clone()
+    plain[0, 40:50] = plain[2, 60] = plain[1, 20] = -100
+
+    def run(lab):
+        logp, _, mask = model.token_logprobs(ids, lab)
+        loss, step = policy_loss(logp, logp.detach() - 0.1, torch.ones(4, device="cuda:0"), mask)
+        loss.backward()
+        got = [logp.detach(), mask, loss.detach(), step.tokens, *grads_of(model)]
+        model.zero_grad(set_to_none=True)
+        return got
+
+    got, want = run(odd), run(plain)
+    assert all(map(torch.equal, got, want)) and int(want[1].sum()) == int(want[3])
