@@ -118,7 +118,7 @@ preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lane
       slope = cfg.beta * (eps * sigmoid(u) - (1.0 - eps) * sigmoid(-u));
     } else if (cfg.loss_type == 1) {
       total += u != u ? u : fmax(0.0, 1.0 - u);
-      slope = u < 1.0 ? -cfg.beta : u - u;             // 0, or NaN where u is
+      slope = u < 1.0 ? -cfg.beta : u != u ? u : 0.0;   // u may be +inf
     } else {
       const double off = d - 0.5 / cfg.beta;
       total += off * off;

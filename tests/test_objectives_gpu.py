@@ -584,3 +584,33 @@ def test_opcheck(cuda, name):
     # places they leave unwritten: the schema, fake and registration checks apply
     tests = ("test_schema", "test_autograd_registration", "test_faketensor")
     torch.library.opcheck(getattr(torch.ops.qlora_b200, name).default, args, test_utils=tests)
+
+
+def test_a_rejected_sequence_that_cannot_occur(cuda):
+    """A counted token of log-probability -inf in the rejected sequence: the pair is infinitely far
+    apart, its loss 0 and its gradients 0, whatever the loss's slope elsewhere; the other pair
+    keeps its own."""
+    from hackathon_b200.preference import preference_loss
+    x = torch.tensor([[-2.0, -1.0], [-1.0, -3.0], [-math.inf, -1.0], [-2.0, -1.0]], device=cuda)
+    alone = torch.tensor([[-1.0, -3.0], [-2.0, -1.0]], device=cuda)
+    for kind in ("sigmoid", "hinge"):
+        for eps in (0.0, 0.2) if kind == "sigmoid" else (0.0,):
+            leaf, one = x.clone().requires_grad_(), alone.clone().requires_grad_()
+            loss, step = preference_loss(leaf, None, None, 0.5, kind, eps, denominator=1.0)
+            want, _ = preference_loss(one, None, None, 0.5, kind, eps, denominator=1.0)
+            (g,) = torch.autograd.grad(loss, leaf)
+            (wg,) = torch.autograd.grad(want, one)
+            assert torch.isfinite(g).all() and float(step.rejected_rewards[0]) == -math.inf
+            assert torch.equal(g[[1, 3]], wg)
+            if eps == 0.0:
+                assert torch.equal(loss.detach(), want.detach()) and not g[[0, 2]].any()
+            else:           # label smoothing: the flipped label costs infinitely much
+                assert float(loss.detach()) == math.inf
+                assert torch.equal(g[[0, 2]], torch.tensor([[0.1], [-0.1]], device=cuda)
+                                   .expand(2, 2))
+    # an infinitely better rejected one: an infinite loss with a finite slope
+    y = torch.tensor([[-math.inf], [-2.0]], device=cuda, requires_grad=True)
+    for kind in ("sigmoid", "hinge"):
+        loss, _ = preference_loss(y, loss_type=kind, beta=0.5)
+        (g,) = torch.autograd.grad(loss, y)
+        assert float(loss.detach()) == math.inf and g.flatten().tolist() == [-0.5, 0.5]
