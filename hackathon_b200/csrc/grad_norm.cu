@@ -144,7 +144,7 @@ grad_norm_kernel(const __grid_constant__ Table<K> table, double* __restrict__ pa
 }
 
 // The norm from the partials, the same in every thread of every CTA.
-__device__ double total_norm(const double* __restrict__ partials, int n, int p, double* scratch) {
+__device__ double total_norm(const double* partials, int n, int p, double* scratch) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < n; i += blockDim.x)
     acc = p == 0 ? join<0>(acc, partials[i]) : acc + partials[i];
@@ -153,8 +153,7 @@ __device__ double total_norm(const double* __restrict__ partials, int n, int p, 
 }
 
 __global__ void __launch_bounds__(kThreads)
-grad_norm_total_kernel(const double* __restrict__ partials, int n, int p,
-                       float* __restrict__ norm) {
+grad_norm_total_kernel(const double* partials, int n, int p, float* __restrict__ norm) {
   qb::await_previous();
   __shared__ double scratch[32];
   const double v = total_norm(partials, n, p, scratch);
@@ -192,8 +191,8 @@ __device__ __forceinline__ void scale_part(T* p, int len, float coef) {
 
 template <int K>
 __global__ void __launch_bounds__(kThreads)
-grad_clip_kernel(const __grid_constant__ Table<K> table, const double* __restrict__ partials,
-                 int n, int p, double max_norm, float* __restrict__ norm) {
+grad_clip_kernel(const __grid_constant__ Table<K> table, const double* partials, int n, int p,
+                 double max_norm, float* __restrict__ norm) {
   qb::await_previous();
   __shared__ double scratch[32];
   const double v = total_norm(partials, n, p, scratch);

@@ -296,8 +296,7 @@ token_logprobs_kernel(const T* __restrict__ logits, Rows rows, int vocab, int sp
 template <typename T>
 __global__ void __launch_bounds__(256)
 token_logprobs_merge_kernel(const T* __restrict__ logits, Rows rows, int64_t n, int vocab,
-                            int spans, float inv_t, Outputs out,
-                            const float4* __restrict__ partials) {
+                            int spans, float inv_t, Outputs out, const float4* partials) {
   qb::await_previous();
   const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= n) return;

@@ -157,7 +157,7 @@ static_assert(kObjPerThread * 32 < 1024, "a warp's counts are packed in ten bits
 // the shares of the tokens held by the lower and by the upper border. weight: one number (token),
 // or one per row.
 __global__ void __launch_bounds__(1024)
-policy_total_kernel(const Record* __restrict__ records, int chunks, int lanes, int64_t rows,
+policy_total_kernel(const Record* records, int chunks, int lanes, int64_t rows,
                     Params par, const double* __restrict__ denom_dev, float* __restrict__ loss,
                     float* __restrict__ stats, float* __restrict__ weight) {
   qb::await_previous();

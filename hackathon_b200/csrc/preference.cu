@@ -71,7 +71,7 @@ __device__ double sigmoid(double x) {
 
 // One CTA: a group of lanes per pair, the rows' records added in a fixed order.
 __global__ void __launch_bounds__(1024)
-preference_pairs_kernel(const Record* __restrict__ records, int chunks, int lanes, int64_t pairs,
+preference_pairs_kernel(const Record* records, int chunks, int lanes, int64_t pairs,
                         const void* __restrict__ ref_row, bool ref_row_double,
                         qb_preference_config cfg, const double* __restrict__ denom_dev,
                         float* __restrict__ loss, float* __restrict__ rewards,

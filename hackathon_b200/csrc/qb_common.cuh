@@ -142,7 +142,9 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // A second launch that follows up on the first (programmatic dependent launch): it is set up while
 // the first still runs, once every CTA of that one has called release_next(), and its own CTAs
 // call await_previous() before they touch memory. Only for a kernel directly behind the one it
-// follows up on.
+// follows up on. What the first writes and the second reads comes in by a pointer without
+// __restrict__: the second's CTAs are alive while it is written, and const __restrict__ would
+// promise memory nobody writes meanwhile - loads ahead of the wait, or by the non-coherent path.
 
 __device__ __forceinline__ void release_next() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -351,3 +351,31 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
         with pytest.raises(RuntimeError, match="qb_thing failed .status 1.: the reason"):
             _lib.call_on(torch.device("cuda", index), "qb_thing")
     assert entered == [1, None, 1, None]
+
+
+def test_second_launches_do_not_promise_read_only_memory():
+    """A kernel that starts before the launch it follows has finished (await_previous) reads what
+    that one writes: none of those pointers may be declared __restrict__, which would allow loads
+    ahead of the wait and through the non-coherent path. Inputs older than both launches may."""
+    import os
+    import re
+    root = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    written = {"partials", "records"}
+    found = 0
+    for name in sorted(os.listdir(root)):
+        if not name.endswith(".cu"):
+            continue
+        with open(os.path.join(root, name)) as f:
+            text = f.read()
+        for part in re.split(r"__global__", text)[1:]:
+            head, _, body = part.partition("{")
+            if "await_previous()" not in body.split("\n}\n")[0]:
+                continue
+            params = re.sub(r"\s+", " ", head[head.index("_kernel"):])
+            names = {p: decl for decl in params.split(",")
+                     for p in written if re.search(rf"\b{p}\b", decl)}
+            assert names, f"{name}: {params}"
+            for decl in names.values():
+                assert "__restrict__" not in decl, f"{name}: {decl}"
+            found += 1
+    assert found == 5
