@@ -31,23 +31,25 @@ F32, F64 = torch.float32, torch.float64
 _library = torch.library.Library(NS, "FRAGMENT")
 _ops = getattr(torch.ops, NS)
 _below_autograd = torch._C._AutoDispatchBelowAutograd
+transformed = torch._C._are_functorch_transforms_active
+_NATIVE = frozenset((torch.Tensor, torch.nn.Parameter, float, int, bool, type(None), torch.dtype))
 
 
-def _plain(t):
-    """A tensor the dispatcher would hand to the CUDA kernel as it is: no subclass (fake and
-    functional tensors are), no mode that wants to see the op."""
-    return type(t) in _PLAIN and t.is_cuda and torch._C._len_torch_dispatch_stack() == 0
-
-
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+def _plain(args):
+    """A call the dispatcher would hand to the CUDA kernel as it is: no tensor subclass (fake and
+    functional tensors are) or symbolic number among the arguments, no mode that wants to see the
+    op, and no function transform, whose tensors are of the plain type and hold no memory."""
+    return (_NATIVE.issuperset(map(type, args)) and args[0].is_cuda
+            and torch._C._len_torch_dispatch_stack() == 0 and not transformed())
 
 
 def _register(schema, fake, function=None):
     """Registers the decorated function as the CUDA kernel of the op `schema` declares, with its
     fake implementation; `function`: the autograd.Function that runs it when the first argument
-    asks for a gradient. Returns what calls the op, with .below for the call below autograd. On
-    plain CUDA tensors (_plain of the first argument) both go to the kernel without the
-    dispatcher, whose boxing of the arguments took 5 to 9 us of a call."""
+    asks for a gradient. Returns what calls the op, with .below for the call below autograd. A
+    plain call (_plain) goes to the kernel without the dispatcher, whose boxing of the arguments
+    took 5 to 9 us of it. Under torch.vmap the dispatcher takes the op to each element; the
+    transforms that differentiate refuse an autograd.Function of this kind by name."""
     name = schema[:schema.index("(")]
 
     def register(kernel):
@@ -57,7 +59,7 @@ def _register(schema, fake, function=None):
         op = getattr(_ops, name).default
 
         def below(*args):
-            if _plain(args[0]):
+            if _plain(args):
                 return kernel(*args)
             with _below_autograd():
                 return op(*args)
@@ -68,7 +70,9 @@ def _register(schema, fake, function=None):
             return below(*args)
 
         def call(*args):
-            return op(*args) if torch.compiler.is_compiling() else autograd(*args)
+            if torch.compiler.is_compiling() or transformed():
+                return op(*args)
+            return autograd(*args)
 
         if function is not None:
             _library.impl(name, autograd, "Autograd")

@@ -3,7 +3,7 @@
 import torch
 
 from . import _lib
-from .objective_ops import constant, divisor, logp_matrix, mask_bytes, policy
+from .objective_ops import constant, divisor, logp_matrix, mask_bytes, policy, transformed
 
 REDUCTIONS = ("token", "sequence")
 
@@ -78,7 +78,8 @@ def policy_loss(logp, old_logp, advantages, mask=None, ref_logp=None, clip_low=0
                          f"{tuple(logp.shape)}")
     mask = mask_bytes("policy_loss", mask, logp)
     denom, divide_by = divisor("policy_loss", denominator, logp.device)
-    with_grad = torch.is_grad_enabled() and logp.requires_grad
+    # a tensor inside a function transform does not say whether the one it stands for asks for one
+    with_grad = torch.is_grad_enabled() and (logp.requires_grad or transformed())
     loss, state, _ = policy(
         logp.to(dtype).contiguous(),
         None if old_logp is None else old_logp.to(dtype).contiguous(),

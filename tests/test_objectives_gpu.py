@@ -614,3 +614,59 @@ def test_a_rejected_sequence_that_cannot_occur(cuda):
         loss, _ = preference_loss(y, loss_type=kind, beta=0.5)
         (g,) = torch.autograd.grad(loss, y)
         assert float(loss.detach()) == math.inf and g.flatten().tolist() == [-0.5, 0.5]
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+@pytest.mark.parametrize("dim", [0, 1])
+def test_batched_calls(cuda, dim):
+    """Under torch.vmap every function gives each element's own results and gradients; the other
+    function transforms, which need more than the ops have, are refused by name."""
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+    logp, mask, randn = draw(cuda, 12, 50, torch.float32, 95)
+    logp, mask = logp.view(3, 4, 50), mask.view(3, 4, 50)
+    old, adv = logp + 0.2 * randn(3, 4, 50), randn(3, 4)
+    z, t = randn(3, 4, 700), torch.arange(12, device=cuda).view(3, 4)
+
+    def one(x, m, o, a, logits, target):
+        p, _ = preference_loss(x, m, o)
+        q, step = policy_loss(x, o, a, m, o, kl_coef=0.1)
+        lp, en = token_logprobs(logits, target, 0.9, True)
+        return p, q, step.kl, lp, en
+
+    args = [logp, mask, old, adv, z, t]
+    want = [torch.stack(v) for v in zip(*(one(*(a[i] for a in args)) for i in range(3)))]
+    moved = [a.movedim(0, dim) for a in args]
+    got = torch.vmap(one, in_dims=dim)(*moved)
+    assert all(map(torch.equal, got, want))
+
+    def total(x, logits):
+        p, q, _, lp, en = torch.vmap(one)(x, mask, old, adv, logits, t)
+        return (p + q).sum() + (lp - en).sum()
+
+    leaf, zl = logp.clone().requires_grad_(), z.clone().requires_grad_()
+    got = torch.autograd.grad(total(leaf, zl), (leaf, zl))
+    for i in range(3):
+        x, y = logp[i].clone().requires_grad_(), z[i].clone().requires_grad_()
+        p, q, _, lp, en = one(x, mask[i], old[i], adv[i], y, t[i])
+        wx, wy = torch.autograd.grad(p + q + (lp - en).sum(), (x, y))
+        assert torch.equal(got[0][i], wx) and torch.equal(got[1][i], wy)
+    with pytest.raises(RuntimeError, match="setup_context"):
+        torch.func.grad(lambda x: preference_loss(x)[0])(logp[0])
+
+
+def test_tensor_subclasses_reach_their_own_dispatch(cuda):
+    """A subclass anywhere among the arguments takes the call to its __torch_dispatch__."""
+    from torch.testing._internal.two_tensor import TwoTensor
+
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.preference import preference_loss
+    logp, mask, randn = draw(cuda, 4, 30, torch.float32, 96)
+    z, t = randn(4, 90), torch.tensor([3, -100, 5, 89], device=cuda)
+    got = token_logprobs(z, TwoTensor(t, t.flip(0)))
+    assert torch.equal(got.a, token_logprobs(z, t))
+    assert torch.equal(got.b, token_logprobs(z, t.flip(0)))
+    got, _ = preference_loss(logp, TwoTensor(mask, mask.flip(0)))
+    assert torch.equal(got.a, preference_loss(logp, mask)[0])
+    assert torch.equal(got.b, preference_loss(logp, mask.flip(0))[0])
