@@ -32,15 +32,18 @@ _library = torch.library.Library(NS, "FRAGMENT")
 _ops = getattr(torch.ops, NS)
 _below_autograd = torch._C._AutoDispatchBelowAutograd
 transformed = torch._C._are_functorch_transforms_active
+_profiled = torch.autograd._profiler_enabled
 _NATIVE = frozenset((torch.Tensor, torch.nn.Parameter, float, int, bool, type(None), torch.dtype))
 
 
 def _plain(args):
     """A call the dispatcher would hand to the CUDA kernel as it is: no tensor subclass (fake and
     functional tensors are) or symbolic number among the arguments, no mode that wants to see the
-    op, and no function transform, whose tensors are of the plain type and hold no memory."""
+    op, no profiler that records it by its name, and no function transform, whose tensors are of
+    the plain type and hold no memory."""
     return (_NATIVE.issuperset(map(type, args)) and args[0].is_cuda
-            and torch._C._len_torch_dispatch_stack() == 0 and not transformed())
+            and torch._C._len_torch_dispatch_stack() == 0 and not transformed()
+            and not _profiled())
 
 
 def _register(schema, fake, function=None):

@@ -670,3 +670,20 @@ def test_tensor_subclasses_reach_their_own_dispatch(cuda):
     got, _ = preference_loss(logp, TwoTensor(mask, mask.flip(0)))
     assert torch.equal(got.a, preference_loss(logp, mask)[0])
     assert torch.equal(got.b, preference_loss(logp, mask.flip(0))[0])
+
+
+def test_profilers_see_the_ops_by_name(cuda):
+    from torch.profiler import ProfilerActivity, profile
+
+    from hackathon_b200.logprobs import token_logprobs
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+    logp, mask, randn = draw(cuda, 4, 30, torch.float32, 97)
+    z, t = randn(4, 90).requires_grad_(), torch.arange(4, device=cuda)
+    leaf = logp.requires_grad_()
+    with profile(activities=[ProfilerActivity.CPU]) as prof:
+        total = token_logprobs(z, t).sum() + preference_loss(leaf, mask)[0] \
+            + policy_loss(leaf, None, randn(4), mask)[0]
+        total.backward()
+    seen = {e.key for e in prof.key_averages()}
+    assert {f"qlora_b200::{name}" for name in NAMES} <= seen
