@@ -14,6 +14,7 @@ from operator import attrgetter
 import torch
 
 from . import _lib
+from .objective_ops import refuse_tangents
 
 _ORDERS = {1.0: 1, 2.0: 2, float("inf"): 0}
 _Tensor = torch.Tensor
@@ -89,6 +90,7 @@ def grad_norm(tensors, norm_type=2.0):
     tensors = [tensors] if isinstance(tensors, _Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
+    refuse_tangents("grad_norm", tensors)
     dev, ptrs, sizes, tags, copies = _table("grad_norm", tensors)
     return _run("qb_grad_norm", dev, ptrs, sizes, tags, order)
 
@@ -110,6 +112,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     grads = [g for g in map(_grad_of, parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
+    refuse_tangents("clip_grad_norm_", grads)
     dev, ptrs, sizes, tags, copies = _table("clip_grad_norm_", grads)
     for t, _ in copies:
         if 0 in (s for n, s in zip(t.shape, t.stride()) if n > 1):

@@ -49,6 +49,7 @@ def linear_token_logprobs(hidden, weight, target, chunk_rows=CHUNK_ROWS):
             or target.shape != hidden.shape[:-1]):
         raise ValueError(f"linear_token_logprobs: hidden {tuple(hidden.shape)} and weight "
                          f"{tuple(weight.shape)} for target {tuple(target.shape)}")
+    objective_ops.refuse_tangents("linear_token_logprobs", (hidden, weight))
     matmul_dtype = _common.autocast_dtype() or torch.promote_types(hidden.dtype, weight.dtype)
     _, token_loss, entropy, _ = FusedLinearCrossEntropy.apply(hidden, weight, target, 1,
                                                               matmul_dtype, chunk_rows)

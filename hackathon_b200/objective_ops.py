@@ -22,6 +22,7 @@ workspace.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -46,6 +47,21 @@ def _plain(args):
             and not _profiled())
 
 
+def _has_tangent(t):
+    if not isinstance(t, torch.Tensor):
+        return False
+    while torch._C._functorch.is_batchedtensor(t):     # a batch's tangent is its base's
+        t = torch._C._functorch.get_unwrapped(t)
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
+def refuse_tangents(what, tensors):
+    """The kernels have no forward-mode derivative: inside a forward-mode level an input with a
+    tangent is refused (a result without its tangent would be a constant)."""
+    if forward_ad._current_level >= 0 and any(map(_has_tangent, tensors)):
+        raise NotImplementedError(f"{what}: no forward-mode derivative, and an input has a tangent")
+
+
 def _register(schema, fake, function=None):
     """Registers the decorated function as the CUDA kernel of the op `schema` declares, with its
     fake implementation; `function`: the autograd.Function that runs it when the first argument
@@ -68,6 +84,7 @@ def _register(schema, fake, function=None):
                 return op(*args)
 
         def autograd(*args):
+            refuse_tangents(f"{NS}::{name}", args)
             if function is not None and torch.is_grad_enabled() and args[0].requires_grad:
                 return function.apply(*args)
             return below(*args)

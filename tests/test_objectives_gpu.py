@@ -687,3 +687,33 @@ def test_profilers_see_the_ops_by_name(cuda):
         total.backward()
     seen = {e.key for e in prof.key_averages()}
     assert {f"qlora_b200::{name}" for name in NAMES} <= seen
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    """No forward-mode derivative: an input with a tangent is refused, not answered without it."""
+    import torch.autograd.forward_ad as fwad
+
+    from hackathon_b200.grad_norm import clip_grad_norm_, grad_norm
+    from hackathon_b200.logprobs import linear_token_logprobs, token_logprobs
+    from hackathon_b200.policy import policy_loss
+    from hackathon_b200.preference import preference_loss
+    logp, mask, randn = draw(cuda, 4, 64, torch.float32, 98)
+    z, t, w, a = randn(4, 64), torch.arange(4, device=cuda), randn(80, 64), randn(4)
+    p = torch.nn.Parameter(randn(5))
+    calls = [(logp, lambda x: preference_loss(x, mask)), (logp, lambda x: policy_loss(x, x, a)),
+             (logp, lambda x: policy_loss(logp, x, a)), (logp, lambda x: preference_loss(logp, mask, x)),
+             (z, lambda x: token_logprobs(x, t)), (z, lambda x: linear_token_logprobs(x, w, t)),
+             (w, lambda x: linear_token_logprobs(z, x, t)), (z, grad_norm)]
+    for x, fn in calls:
+        with fwad.dual_level():
+            for y in (x, x.clone().requires_grad_()):
+                dual = fwad.make_dual(y, torch.ones_like(x))
+                with pytest.raises((NotImplementedError, ValueError)):
+                    fn(dual)
+            fn(x)                               # plain inputs are served there as anywhere
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(fn, (x,), (torch.ones_like(x),))
+    with fwad.dual_level():
+        p.grad = fwad.make_dual(randn(5), torch.ones(5, device=cuda))
+        with pytest.raises(NotImplementedError):
+            clip_grad_norm_(p, 1.0)
