@@ -291,13 +291,13 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
     n, cols = logp.shape
     dev = logp.device
     here = logp.get_device()
-    _need(logp.is_contiguous() and _fits(ref, here, logp.dtype, logp.shape)
+    _need(n % 2 == 0 and logp.is_contiguous() and _fits(ref, here, logp.dtype, logp.shape)
           and (ref_row is None or ref_row.dtype in (F32, F64)
                and _fits(ref_row, here, ref_row.dtype, (n,)))
           and _fits(denominator, here, F64, ())
           and _mask_fits(mask, here, logp.shape), "preference",
-          "contiguous tensors on one device: ref in logp's dtype, ref_row fp32 or fp64, bool or "
-          "byte mask, double denominator")
+          "pairs of rows, contiguous tensors on one device: ref in logp's dtype, ref_row fp32 or "
+          "fp64, bool or byte mask, double denominator")
     loss = torch.empty((), dtype=F32, device=dev)
     size, at = preference_state(n, cols)
     state = torch.empty(size, dtype=F32, device=dev)
@@ -320,9 +320,9 @@ def preference(logp, mask, ref, ref_row, denominator, beta, label_smoothing, mar
            lambda state, mask, g, n, cols, dtype: state.new_empty((n, cols), dtype=dtype))
 def preference_bwd(state, mask, g, n, cols, dtype):
     here = state.get_device()
-    _need(state.dtype == F32 and state.is_contiguous() and state.numel() >= 2 * n
+    _need(n % 2 == 0 and state.dtype == F32 and state.is_contiguous() and state.numel() >= 2 * n
           and _fits(g, here, F32, ()) and _mask_fits(mask, here, (n, cols)),
-          "preference_bwd", "state, mask and gradient as the forward has them")
+          "preference_bwd", "pairs of rows; state, mask and gradient as the forward has them")
     out = torch.empty((n, cols), dtype=dtype, device=state.device)
     _lib.call_on(state.device, "qb_preference_bwd", _lib.ptr(mask), state.data_ptr() + 4 * n,
                  g.data_ptr(), n // 2, cols, out.data_ptr(), _lib.tag(dtype),

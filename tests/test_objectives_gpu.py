@@ -717,3 +717,14 @@ def test_forward_mode_tangents_are_refused(cuda):
         p.grad = fwad.make_dual(randn(5), torch.ones(5, device=cuda))
         with pytest.raises(NotImplementedError):
             clip_grad_norm_(p, 1.0)
+
+
+def test_preference_ops_refuse_an_odd_row(cuda):
+    """The kernels read pairs: a row without a partner would be left out of everything."""
+    logp, mask, _ = draw(cuda, 5, 30, torch.float32, 92)
+    ns = torch.ops.qlora_b200
+    with pytest.raises(ValueError, match="preference"):
+        ns.preference(logp, mask, None, None, None, 0.1, 0.0, 0.0, 0.0, 0, False)
+    state, g = torch.zeros(64, device=cuda), torch.ones((), device=cuda)
+    with pytest.raises(ValueError, match="preference_bwd"):
+        ns.preference_bwd(state, mask, g, 5, 30, torch.float32)
