@@ -728,3 +728,29 @@ def test_preference_ops_refuse_an_odd_row(cuda):
     state, g = torch.zeros(64, device=cuda), torch.ones((), device=cuda)
     with pytest.raises(ValueError, match="preference_bwd"):
         ns.preference_bwd(state, mask, g, 5, 30, torch.float32)
+
+
+def test_policy_at_the_borders_rounded_differences(cuda):
+    """Differences whose fp32 value is a border's own rounding: the exact one decides, for the
+    gradient and for the shares. old = +- 7/16 of the border's last place moves it to either side
+    of the border (each is rounded by less) without moving its fp32 value."""
+    from hackathon_b200.policy import policy_loss
+    low, high, delta = math.log1p(-0.2), math.log1p(0.28), math.log(1.6)
+    rows = torch.tensor([low, high, delta], dtype=torch.float64).float()
+    x = rows[:, None].repeat(1, 2).to(cuda)
+    step = (torch.nextafter(rows, torch.full_like(rows, 9.0)) - rows)[:, None].to(cuda) * 7 / 16
+    old = torch.cat([step, -step], 1)
+    exact = x.double() - old.double()
+    assert torch.equal(x - old, x)                              # they tie in fp32 ...
+    edge = torch.tensor([low, high, delta], dtype=torch.float64, device=cuda)[:, None]
+    assert torch.equal(exact < edge, torch.tensor([[True, False]] * 3, device=cuda))
+    for sign in (1.0, -1.0):
+        adv = torch.full((3,), sign, device=cuda)
+        leaf = x.clone().requires_grad_()
+        loss, step = policy_loss(leaf, old, adv, None, None, 0.2, 0.28, 1.6)
+        (g,) = torch.autograd.grad(loss, leaf)
+        below, above, past = exact < low, exact > high, exact > delta
+        live = ~past & (~(below | above) | (below & (sign > 0)) | (above & (sign < 0)))
+        assert torch.equal(g != 0, live)
+        assert float(step.clipped_low) == float((below & (sign < 0)).double().mean().float())
+        assert float(step.clipped_high) == float((above & (sign > 0)).double().mean().float())
