@@ -371,3 +371,35 @@ def test_targets_outside_the_vocabulary_score_nothing(cuda, vocab, dtype, monkey
         broken[at] = math.nan
         lost = run(t, broken)
         assert torch.equal(lost[0], want[0]) and torch.equal(lost[1], want[1])
+
+
+@pytest.mark.parametrize("temperature", [0.7, 0.9, 1.0, 2.5])
+def test_gradient_of_a_nearly_certain_token(cuda, temperature):
+    """A target of probability 1 - q with q about 2^-20 has the gradient g q / T. Its only rival's
+    logit d is one whose scaled exponent is a whole number, so the row's sum 1 + 2^-k is exact and
+    q is good to 4 u |d / T| + 4 u (the exponent's scale and product, 2^y); the gradient's products
+    add 4 u: 2^-16 relative covers d / T of 14. One of g / T and -g p / T, each rounded by itself
+    before they cancel, is off by u / q: 2^-4."""
+    import numpy as np
+
+    from hackathon_b200.logprobs import token_logprobs
+    one = np.float32(1)
+    c = (one / np.float32(temperature)) * np.float32(1.4426950408889634)
+    for k in (18, 20):
+        d = np.float32(-k / np.float64(c))
+        for _ in range(40):
+            if d * c == -k:
+                break
+            d = np.nextafter(d, np.float32(-100 if d * c > -k else 100))
+        assert d * c == -k
+        for v, label, rival in ((2000, 700, 3), (2001, 2000, 5), (5, 2, 4), (40001, 9, 40000)):
+            z = torch.full((4, v), -math.inf, device=cuda)
+            z[:, label], z[:, rival] = 0.0, float(d)
+            t = torch.full((4,), label, device=cuda)
+            gl = torch.tensor([1.0, 0.37, -2.9, 1e-3], device=cuda)
+            leaf = z.requires_grad_()
+            (g,) = torch.autograd.grad(token_logprobs(leaf, t, temperature), leaf, gl)
+            x = math.exp(float(d) / temperature)
+            want = gl.double() / temperature * (x / (1 + x))
+            assert bool(((g[:, label].double() - want).abs() <= 2.0 ** -16 * want.abs()).all())
+            assert bool(((g[:, rival].double() + want).abs() <= 2.0 ** -16 * want.abs()).all())
