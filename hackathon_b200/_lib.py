@@ -164,7 +164,7 @@ class KernelTimer:
             d["launches"] += 1
             d["kernels"] += kernels
             d["ms_total"] += s.elapsed_time(e)
-            d["bytes"] += nbytes
+            d["bytes"] += nbytes() if callable(nbytes) else nbytes
             d["flops"] += flops
         return out
 
@@ -173,14 +173,15 @@ _timer = None
 
 
 def timing():
-    """True while a KernelTimer is active (a caller whose work figures cost time to add up asks)."""
+    """True while a KernelTimer is active (a caller that keeps something for its figures asks)."""
     return _timer is not None
 
 
 def call(name, *args, work=(0, 0), kernels=1):
     """Calls a C-ABI entry point; raises RuntimeError with the library's message on failure.
     `work` = (algorithmic bytes, flops) of the call and `kernels` the kernels it launches,
-    recorded when a KernelTimer is active."""
+    recorded when a KernelTimer is active. Bytes that depend on the data are a function, called
+    once the device is done."""
     lib = load()
     timer = _timer
     if timer is not None:
@@ -189,7 +190,8 @@ def call(name, *args, work=(0, 0), kernels=1):
         s.record()
         status = getattr(lib, name)(*args)
         e.record()
-        timer.records.append((name, s, e, int(work[0]), int(work[1]), int(kernels)))
+        nbytes = work[0] if callable(work[0]) else int(work[0])
+        timer.records.append((name, s, e, nbytes, int(work[1]), int(kernels)))
     else:
         status = getattr(lib, name)(*args)
     if status != 0:

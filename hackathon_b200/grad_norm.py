@@ -69,15 +69,23 @@ def _table(what, tensors):
     return tensors[0].device, ptrs, array("q", map(_Tensor.numel, tensors)), tags, copies
 
 
-def _run(name, dev, ptrs, sizes, tags, order, *limit, passes=1):
+def _run(name, dev, ptrs, sizes, tags, order, max_norm=None):
     n = len(ptrs)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     doubles = _lib.load().qb_grad_norm_workspace(n)
     work = torch.empty(doubles, dtype=torch.float64, device=dev)
-    _lib.call_on(dev, name, ptrs.buffer_info()[0], sizes.buffer_info()[0], tags,
-                 n, order, *limit, work.data_ptr(), doubles, norm.data_ptr(), kernels=2,
-                 work=(passes * sum(s * (4 if t == _lib.F32 else 2)
-                                    for s, t in zip(sizes, tags)) if _lib.timing() else 0, 0))
+    limit = () if max_norm is None else (array("d", [max_norm]),)
+
+    def moved():                     # a kernel timer asks when the norm is known
+        once = sum(s * (4 if t == _lib.F32 else 2) for s, t in zip(sizes, tags))
+        scaled = limit and not max_norm >= float(seen) + 1e-6
+        return 3 * once if scaled else once
+
+    _lib.call_on(dev, name, ptrs.buffer_info()[0], sizes.buffer_info()[0], tags, n, order,
+                 *(a.buffer_info()[0] for a in limit), work.data_ptr(), doubles, norm.data_ptr(),
+                 kernels=2, work=(moved, 0))
+    # the caller may write to the norm it gets
+    seen = norm.clone() if limit and _lib.timing() else norm
     return norm
 
 
@@ -122,8 +130,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         norm = _run("qb_grad_norm", dev, ptrs, sizes, tags, order)
         if not torch.isfinite(norm):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {norm.item()}")
-    limit = array("d", [max_norm])
-    norm = _run("qb_grad_clip", dev, ptrs, sizes, tags, order, limit.buffer_info()[0], passes=3)
+    norm = _run("qb_grad_clip", dev, ptrs, sizes, tags, order, max_norm)
     for t, c in copies:
         t.copy_(c)
     torch.autograd.graph.increment_version(grads)

@@ -211,3 +211,24 @@ def test_same_bits_stream_graph_and_version(cuda):
         graph.replay()
         assert abs(float(out) - norm64(src, 2.0)) <= 2 * U * norm64(src, 2.0)
         assert abs(norm64(work, 2.0) - 0.5) < 1e-5
+
+
+def test_timer_counts_the_bytes_that_moved(cuda):
+    """A kernel timer's bytes: one pass for a norm and for a clipping within the limit, the norm's
+    read and the scaling's read and write where it scales."""
+    from hackathon_b200 import _lib
+    from hackathon_b200.grad_norm import clip_grad_norm_, grad_norm
+    grads = [torch.ones(300, device=cuda), torch.ones(100, device=cuda, dtype=torch.bfloat16)]
+    size, ps = 300 * 4 + 100 * 2, params_of(grads)
+    for limit, passes in ((1e3, 1), (1.0, 3), (math.inf, 1), (0.0, 3)):
+        for g in grads:
+            g.fill_(1.0)
+        with _lib.KernelTimer() as timer:
+            clip_grad_norm_(ps, limit).zero_()          # the caller's to write to
+        assert timer.summary()["qb_grad_clip"]["bytes"] == passes * size
+    grads[0][7] = math.nan
+    with _lib.KernelTimer() as timer:
+        grad_norm(grads)
+        clip_grad_norm_(ps, 1e3)
+    both = timer.summary()
+    assert both["qb_grad_norm"]["bytes"] == size and both["qb_grad_clip"]["bytes"] == 3 * size
