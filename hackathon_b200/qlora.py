@@ -631,6 +631,8 @@ class QwenQLoRA(torch.nn.Module):
         self.gemm_masks = True
         self._rope = {}
         self.step_seed = 0
+        # the last step's gradient norm before clipping (on the device), None if it did not clip
+        self.grad_norm = None
         # the bf16 adapter operands of every projection, rebuilt by one launch per forward
         from .lora import AdapterShadow
         self.adapter_shadow = AdapterShadow(
@@ -739,7 +741,7 @@ def _update(model, opt, loss, grad_sync, max_grad_norm):
     loss.backward()
     if grad_sync is not None:
         grad_sync()
-    if max_grad_norm is not None:
+    model.grad_norm = None if max_grad_norm is None else \
         clip_grad_norm_(model.adapter_parameters(), max_grad_norm)
     opt.step()
     # with a gradient sync the .grad tensors are views into its flat buffer and stay; without
@@ -753,7 +755,7 @@ def train_step(model, opt, input_ids, labels, grad_sync=None, num_items_in_batch
                max_grad_norm=None):
     """One optimizer step on the next-token loss; returns the loss tensor (on the device, not
     synchronised). max_grad_norm: the adapters' gradients are scaled to that norm first when
-    theirs is larger."""
+    theirs, kept as model.grad_norm, is larger."""
     model.train()
     loss, _ = model(input_ids, labels, num_items_in_batch=num_items_in_batch)
     return _update(model, opt, loss, grad_sync, max_grad_norm)

@@ -344,3 +344,24 @@ def test_labels_outside_the_vocabulary_are_not_scored(cuda):
 
     got, want = run(odd), run(plain)
     assert all(map(torch.equal, got, want)) and int(want[1].sum()) == int(want[3])
+
+
+def test_steps_keep_the_norm_they_clipped_by(cuda):
+    """model.grad_norm: the gradients' norm before clipping, None after a step without clipping."""
+    from hackathon_b200.qlora import train_step
+    model, shape = tiny()
+    ids, labels = batch(shape, 4, 64)
+    params = model.adapter_parameters()
+    opt = torch.optim.SGD(params, lr=0.0)
+    seen = []
+    opt.register_step_pre_hook(lambda *_: seen.append(
+        math.sqrt(sum(float(p.grad.double().square().sum()) for p in params))))
+    assert model.grad_norm is None
+    train_step(model, opt, ids, labels, max_grad_norm=1e6)
+    norm = float(model.grad_norm)
+    assert not model.grad_norm.requires_grad and abs(norm - seen[0]) <= 4 * U * seen[0]
+    train_step(model, opt, ids, labels, max_grad_norm=norm / 4)
+    assert float(model.grad_norm) == norm and abs(seen[1] - norm / 4) <= 1e-3 * norm
+    assert "grad_norm" not in model.state_dict()
+    train_step(model, opt, ids, labels)
+    assert model.grad_norm is None
