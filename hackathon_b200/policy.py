@@ -54,8 +54,8 @@ def policy_loss(logp, old_logp, advantages, mask=None, ref_logp=None, clip_low=0
     clip_high = clip_low if clip_high is None else float(clip_high)
     if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float("inf"):
         raise ValueError(f"policy_loss: clip range {clip_low}, {clip_high}")
-    delta = 0.0 if delta is None else float(delta)
-    if delta and not 1.0 + clip_high < delta < float("inf"):
+    delta = None if delta is None else float(delta)
+    if delta is not None and not 1.0 + clip_high < delta < float("inf"):
         raise ValueError(f"policy_loss: delta {delta} is not above 1 + clip_high")
     kl_coef = float(kl_coef)
     if not abs(kl_coef) < float("inf") or (kl_coef and ref_logp is None):
@@ -85,5 +85,5 @@ def policy_loss(logp, old_logp, advantages, mask=None, ref_logp=None, clip_low=0
         None if old_logp is None else old_logp.to(dtype).contiguous(),
         advantages.to(torch.float32), mask,
         None if ref_logp is None else ref_logp.to(dtype).contiguous(), denom, clip_low, clip_high,
-        delta, kl_coef, divide_by, reduction == "sequence", with_grad)
+        delta or 0.0, kl_coef, divide_by, reduction == "sequence", with_grad)
     return loss, PolicyStep(state)

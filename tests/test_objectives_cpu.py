@@ -379,3 +379,13 @@ def test_second_launches_do_not_promise_read_only_memory():
                 assert "__restrict__" not in decl, f"{name}: {decl}"
             found += 1
     assert found == 5
+
+
+def test_policy_second_border_of_zero_is_refused():
+    """None is no second border; 0 is one below the others, not another word for None."""
+    def run(e):
+        for bad in (0, 0.0, -0.0):
+            with pytest.raises(ValueError, match="delta"):
+                policy_loss(e(4, 6), e(4, 6), e(4), delta=bad)
+        policy_loss(e(4, 6), e(4, 6), e(4), delta=None)
+    _fake_cuda(run)
