@@ -464,7 +464,10 @@ def divisor(what, denominator, device):
     if torch.is_tensor(denominator):
         if denominator.numel() != 1:
             raise ValueError(f"{what}: the denominator is one number")
-        return denominator.detach().reshape(()).to(device=device, dtype=torch.float64), 0.0
+        if denominator.requires_grad:
+            raise ValueError(f"{what}: the denominator is a constant of the objective (no gradient "
+                             "flows into it); pass it detached")
+        return denominator.reshape(()).to(device=device, dtype=torch.float64), 0.0
     value = float(denominator)
     if not 0.0 < value < float("inf"):
         raise ValueError(f"{what}: denominator {denominator} is not positive")

@@ -389,3 +389,15 @@ def test_policy_second_border_of_zero_is_refused():
                 policy_loss(e(4, 6), e(4, 6), e(4), delta=bad)
         policy_loss(e(4, 6), e(4, 6), e(4), delta=None)
     _fake_cuda(run)
+
+
+def test_denominators_that_ask_for_a_gradient_are_refused():
+    """As every other constant of an objective: its gradient would go nowhere."""
+    def run(e):
+        x, denom = e(4, 6), e((), requires_grad=True)
+        with pytest.raises(ValueError, match="denominator.*detached"):
+            policy_loss(x, x, e(4), denominator=denom)
+        with pytest.raises(ValueError, match="denominator.*detached"):
+            preference_loss(x, denominator=denom)
+        policy_loss(x, x, e(4), denominator=denom.detach())
+    _fake_cuda(run)
