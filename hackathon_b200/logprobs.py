@@ -12,6 +12,11 @@ from . import _common, _lib, objective_ops
 from .cross_entropy import CHUNK_ROWS, FusedLinearCrossEntropy
 
 
+def _whole_numbers(what, target):
+    if target.is_floating_point() or target.is_complex() or target.dtype == torch.bool:
+        raise TypeError(f"{what}: target holds token numbers, got {target.dtype}")
+
+
 def token_logprobs(logits, target, temperature=1.0, with_entropy=False):
     """ln softmax(logits / temperature)[target] per position, fp32, and with_entropy the pair of it
     and the entropy of softmax(logits / temperature). logits [..., V] in fp32, fp16 or bf16,
@@ -26,8 +31,7 @@ def token_logprobs(logits, target, temperature=1.0, with_entropy=False):
                          f"{tuple(target.shape)}")
     if target.device != logits.device:
         raise ValueError(f"token_logprobs: target on {target.device}, logits on {logits.device}")
-    if target.is_floating_point() or target.is_complex() or target.dtype == torch.bool:
-        raise TypeError(f"token_logprobs: target holds token numbers, got {target.dtype}")
+    _whole_numbers("token_logprobs", target)
     temperature = float(temperature)
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"token_logprobs: temperature {temperature} is not in 1e-6 .. 1e6")
@@ -49,6 +53,7 @@ def linear_token_logprobs(hidden, weight, target, chunk_rows=CHUNK_ROWS):
             or target.shape != hidden.shape[:-1]):
         raise ValueError(f"linear_token_logprobs: hidden {tuple(hidden.shape)} and weight "
                          f"{tuple(weight.shape)} for target {tuple(target.shape)}")
+    _whole_numbers("linear_token_logprobs", target)
     objective_ops.refuse_tangents("linear_token_logprobs", (hidden, weight))
     matmul_dtype = _common.autocast_dtype() or torch.promote_types(hidden.dtype, weight.dtype)
     _, token_loss, entropy, _ = FusedLinearCrossEntropy.apply(hidden, weight, target, 1,

@@ -401,3 +401,14 @@ def test_denominators_that_ask_for_a_gradient_are_refused():
             preference_loss(x, denominator=denom)
         policy_loss(x, x, e(4), denominator=denom.detach())
     _fake_cuda(run)
+
+
+def test_linear_token_logprobs_targets_are_whole_numbers():
+    """A target of another kind has no token: refused, as token_logprobs does, not cut off."""
+    def run(e):
+        for dtype in (F32, BF, torch.bool):
+            with pytest.raises(TypeError, match="token numbers"):
+                linear_token_logprobs(e(2, 5, 8), e(30, 8), e(2, 5, dtype=dtype))
+        for dtype in (I64, torch.int32, torch.uint8):
+            linear_token_logprobs(e(2, 5, 8), e(30, 8), e(2, 5, dtype=dtype))
+    _fake_cuda(run)
