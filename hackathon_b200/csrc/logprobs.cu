@@ -173,7 +173,10 @@ __device__ __forceinline__ Stat warp_merge(Stat st, Scale c) {
   return st;
 }
 
-// U vectors of a thread: one maximum and at most one rescaling for all of them.
+// U vectors of a thread: one maximum and at most one rescaling for all of them, and sums of their
+// own that join the thread's at the end. (Added one by one, a thread that holds the row's top token
+// rounds every term at that one's last place: 2.6e-7 instead of 1.2e-7 in the gradient of 999 rows
+// of 50001, at the same time.)
 template <typename T, bool ENT, int U>
 __device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scale c) {
   float m = x[0].top();
@@ -182,7 +185,7 @@ __device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scal
   if (m == -INFINITY) return;    // all banned: nothing to add, and no maximum to subtract
   if (m > st.m) rescale(st, m, c);
   const Pair cc = pair(c.c, c.c);
-  Pair s = pair(st.s, 0.f), t = pair(st.t, 0.f);
+  Pair s = pair(0.f, 0.f), t = pair(0.f, 0.f);
   float lo, hi;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -199,9 +202,9 @@ __device__ __forceinline__ void add_vectors(Stat& st, const Vec<T> (&x)[U], Scal
     }
   }
   halves(s, lo, hi);
-  st.s = lo + hi;
+  st.s += lo + hi;
   halves(t, lo, hi);
-  st.t = lo + hi;
+  st.t += lo + hi;
 }
 
 template <bool ENT>

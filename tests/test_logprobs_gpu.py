@@ -403,3 +403,17 @@ def test_gradient_of_a_nearly_certain_token(cuda, temperature):
             want = gl.double() / temperature * (x / (1 + x))
             assert bool(((g[:, label].double() - want).abs() <= 2.0 ** -16 * want.abs()).all())
             assert bool(((g[:, rival].double() + want).abs() <= 2.0 ** -16 * want.abs()).all())
+
+
+def test_small_terms_beside_the_top_one_count(cuda):
+    """200,000 terms of 0.9 * 2^-24 beside one of 1: each is lost when added to a sum of 1 or more.
+    A thread's batches hold 32 terms in two sums and there are V / 4096 of them, then come about a
+    dozen merges; each such addition is off by 2^-24 at most."""
+    from hackathon_b200.logprobs import token_logprobs
+    v, d = 200_000, -16.75
+    z = torch.full((600, v), d, dtype=torch.bfloat16, device=cuda)     # rows in one span each
+    z[:, 0] = 0.0
+    lp = token_logprobs(z, torch.zeros(600, dtype=torch.int64, device=cuda))
+    want = -math.log1p((v - 1) * math.exp(d))
+    bound = U * (v / 4096 + 16 + 12) + 4 * U * abs(want) + U * 4 * abs(d) * abs(want)
+    assert float((lp.double() - want).abs().max()) <= bound
