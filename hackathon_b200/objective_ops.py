@@ -42,9 +42,8 @@ def _plain(args):
     functional tensors are) or symbolic number among the arguments, no mode that wants to see the
     op, no profiler that records it by its name, and no function transform, whose tensors are of
     the plain type and hold no memory."""
-    return (_NATIVE.issuperset(map(type, args)) and args[0].is_cuda
-            and torch._C._len_torch_dispatch_stack() == 0 and not transformed()
-            and not _profiled())
+    return (_NATIVE.issuperset(map(type, args)) and args[0].is_cuda and not (
+        transformed() or _profiled() or torch._C._len_torch_dispatch_stack()))
 
 
 def _has_tangent(t):
@@ -67,7 +66,7 @@ def _register(schema, fake, function=None):
     fake implementation; `function`: the autograd.Function that runs it when the first argument
     asks for a gradient. Returns what calls the op, with .below for the call below autograd. A
     plain call (_plain) goes to the kernel without the dispatcher, whose boxing of the arguments
-    took 5 to 9 us of it. Under torch.vmap the dispatcher takes the op to each element; the
+    takes 5 to 9 us. Under torch.vmap the dispatcher takes the op to each element; the
     transforms that differentiate refuse an autograd.Function of this kind by name."""
     name = schema[:schema.index("(")]
 
@@ -85,14 +84,19 @@ def _register(schema, fake, function=None):
 
         def autograd(*args):
             refuse_tangents(f"{NS}::{name}", args)
-            if function is not None and torch.is_grad_enabled() and args[0].requires_grad:
+            if torch.is_grad_enabled() and args[0].requires_grad:
                 return function.apply(*args)
             return below(*args)
 
         def call(*args):
-            if torch.compiler.is_compiling() or transformed():
+            if torch.compiler.is_compiling():
                 return op(*args)
-            return autograd(*args)
+            if not _plain(args) or forward_ad._current_level >= 0:
+                refuse_tangents(f"{NS}::{name}", args)
+                return op(*args)
+            if function is not None and torch.is_grad_enabled() and args[0].requires_grad:
+                return function.apply(*args)
+            return kernel(*args)
 
         if function is not None:
             _library.impl(name, autograd, "Autograd")

@@ -754,3 +754,17 @@ def test_policy_at_the_borders_rounded_differences(cuda):
         assert torch.equal(g != 0, live)
         assert float(step.clipped_low) == float((below & (sign < 0)).double().mean().float())
         assert float(step.clipped_high) == float((above & (sign > 0)).double().mean().float())
+
+
+def test_upstream_tangents_are_refused_in_the_backward(cuda):
+    """The gradient's own op has no forward-mode derivative either."""
+    import torch.autograd.forward_ad as fwad
+
+    from hackathon_b200.preference import preference_loss
+    logp, mask, _ = draw(cuda, 4, 30, torch.float32, 99)
+    leaf = logp.requires_grad_()
+    loss, _ = preference_loss(leaf, mask)
+    one = torch.ones((), device=cuda)
+    with fwad.dual_level():
+        with pytest.raises(NotImplementedError, match="preference_bwd"):
+            torch.autograd.grad(loss, leaf, fwad.make_dual(one, one))
