@@ -14,7 +14,7 @@ The functions users call (logprobs.py, preference.py, policy.py) check their arg
 them into the layouts these ops read. The kernels of an objective take a few microseconds at the
 sizes of a batch, so the host's part decides: the ops are registered with torch.library's
 define / impl and an autograd.Function of their own (a preference loss and its gradient took
-239 us of host time through torch.library.custom_op and its generated formula and takes 115 now,
+239 us of host time through torch.library.custom_op and its generated formula and takes 112 now,
 69 of them an empty autograd.Function's), and small outputs share one allocation with the
 workspace.
 """
